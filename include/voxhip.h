@@ -438,6 +438,81 @@ int voxhip_quantize_q8_dev(const float *d_w, int64_t rows, int64_t cols, int8_t 
 int voxhip_quantize_q4_dev(const float *d_w, int64_t rows, int64_t cols, uint8_t *d_q, float *d_scale);
 int voxhip_quantize_act_dev(const float *d_x, int64_t n, int8_t *d_xq, float *d_xs);
 
+/* ---------------------------------------------------------------- paged key/value cache
+ * A cache in pages of one pool for servers whose sequences come and go, with the append of a step's rows and the attention
+ * that reads it. No counterpart in the reference, whose caches are one buffer per sequence. All pointers are device memory,
+ * also those inside the structs, and belong to the caller, who keeps them until the work is done; the structs are read during
+ * the call. The calls are asynchronous on the library's stream: what they read has to be there (voxhip_memcpy_h2d, or
+ * the caller's own stream waited for), and voxhip_sync waits for what they write. Calls of one batch on one stream of work
+ * serialise; the library's own workspace is shared by them all.
+ *
+ * Device contents are not checked by the host. A table entry that names no page of the pool, or row_start / len beyond the
+ * buffers, touches nothing outside them: those keys are left out, those rows not written or of no meaning, and the next
+ * voxhip_sync (or synchronous call) fails. */
+/* One layer's pool: element d of kv head h at position p of a sequence lies at
+ * page * page_stride + h * head_stride + (p % page_size) * pos_stride + d elements of k (and of v), page = the sequence's
+ * table entry p / page_size. Both [pages][kv_heads][page_size][head_dim] and [pages][page_size][kv_heads][head_dim] (and wider
+ * strides) fit. type F16 or BF16; head_dim a multiple of 8 up to 128; page_size a power of two, 8..1024; strides multiples
+ * of 8; k, v aligned to 16 bytes. */
+typedef struct voxhip_paged_kv {
+    void *k, *v;
+    int32_t type, pages, page_size, kv_heads, head_dim;
+    int64_t page_stride, head_stride, pos_stride;
+} voxhip_paged_kv;
+/* A ragged batch: rows row_start[s] .. row_start[s + 1] - 1 of the row buffers (which hold `rows`) belong to sequence s, in
+ * order; len[s] is the number of its keys with those rows among them, so that row i of n stands at position len[s] - n + i.
+ * Sequences without rows are allowed, and so are rows at negative positions (padding in front, len 0: they have no key) and
+ * rows behind the last sequence's (left as they are). pages: [seqs][page_ld]; an entry is read only for positions below
+ * len[s]. max_rows / max_len: at least the largest number of rows and keys of a sequence (they only shape the launch: larger
+ * values cost time). */
+typedef struct voxhip_paged_batch {
+    int32_t seqs, rows, max_rows, max_len;
+    const int32_t *row_start, *len, *pages;
+    int64_t page_ld;
+} voxhip_paged_batch;
+/* Rows [q: heads head_dim | k: kv_heads head_dim | v: kv_heads head_dim] of type F32 or F16 (f16 cache) or BF16 (bf16 cache),
+ * strides multiples of 8, pointers aligned to 16 bytes. q_norm / k_norm [head_dim] (NULL: none): x / sqrt(mean x^2 + eps) * w
+ * per head first. rope [rope_len][rot_dim / 2] (cos, sin) pairs (NULL: no rotation) turns the first rot_dim (a multiple of 8)
+ * dims of q and k, pairs (j, j + rot_dim / 2), or (2 j, 2 j + 1) when interleaved; all in f32, rounded once. */
+typedef struct voxhip_append_rows {
+    int32_t type, heads;
+    const void *qkv;
+    int64_t ld_qkv;
+    void *q;                       /* [rows][ld_q] out: the turned queries, apart from qkv; NULL: k and v only */
+    int64_t ld_q;
+    const float *q_norm, *k_norm;
+    float eps;
+    const float *rope;
+    int32_t rope_len, rot_dim, interleaved;
+} voxhip_append_rows;
+/* Writes the batch's rows into their pages. Pages written by a call belong to one sequence each. Returns 1 or 0. */
+int voxhip_kv_append_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r);
+/* Query rows q [rows][ld_q] and out [rows][ld_out] (may be q) of `heads` heads (a multiple of kv_heads), types as above.
+ * The row at position p of a sequence sees the keys max(0, p - window + 1) (window 0: 0) .. min(len, max(p + 1, prefix[s])) - 1
+ * and takes the mean of their values weighted by softmax of scale q.k, capped to cap tanh(. / cap) (cap 0: not), less
+ * slopes[head] |p - key| (NULL: not). A row that sees no key gets zeros. */
+typedef struct voxhip_attn_rows {
+    int32_t type, heads;
+    const void *q;
+    int64_t ld_q;
+    void *out;
+    int64_t ld_out;
+    float scale, cap;
+    const float *slopes;
+    const int32_t *prefix;
+    int32_t window;
+} voxhip_attn_rows;
+int voxhip_attn_paged_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_attn_rows *r);
+/* The same where sequences seq_start[g] .. seq_start[g + 1] - 1 of group g begin with the same len[g] keys: those are read
+ * from the pages of the group's first sequence, once for all of its rows (the others' table entries for them are not read).
+ * seq_start [groups + 1] never falls; sequences outside every group share nothing. max_len: at least the largest len[g]. */
+typedef struct voxhip_shared_prefix {
+    int32_t groups, max_len;
+    const int32_t *seq_start, *len;
+} voxhip_shared_prefix;
+int voxhip_attn_shared_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_shared_prefix *p,
+                           const voxhip_attn_rows *r);
+
 /* ---------------------------------------------------------------- measurement */
 /* Kernel classes of one decode step, for voxhip_bench_result. */
 enum voxhip_kernel_class {

@@ -2,11 +2,15 @@
 #pragma once
 #include <stdint.h>
 
+#include "vh_paged_index.hpp"
+
 namespace vh {
 
 // The library's range-status word: a kernel whose arithmetic cannot represent a value it was given sets a bit, and
 // the synchronous entry points fail the call when one is set (so the engine computes it on the CPU instead).
-enum : int32_t { kStatusF16Range = 1, kStatusFixRange = 2 };
+// kStatusBadPage / kStatusBadBatch: a page table, or a ragged batch's row_start / len, that names what is not there (the
+// kernel leaves those keys out and touches nothing outside its buffers).
+enum : int32_t { kStatusF16Range = 1, kStatusFixRange = 2, kStatusBadPage = 4, kStatusBadBatch = 8 };
 
 // GEMV input prologues: x as is; RMSNorm(x, gamma); or the merge of split-K attention partials.
 // GEMV prologues; PRO_Q (int path only): the input rows arrive already quantized (k_quant_rows)
@@ -308,5 +312,32 @@ constexpr int kLmMaxN = 8192;  // vocabulary limit of the device RAS sampler (8 
 
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleMaxN = 16384;  // logits per call (keys sorted in LDS)
+
+// The paged cache's append and attention (vh_paged.hpp).
+struct AppendArgs {
+    PagedKv c;
+    PagedBatch b;
+    const void *qkv;
+    void *q;  // or null
+    int64_t ld_qkv, ld_q;
+    const float *qn, *kn, *rope;  // or null
+    int32_t heads, rope_len, rot, interleaved, blocks;
+    float eps;
+    int32_t *status;
+};
+
+struct PagedAttnArgs {
+    PagedKv c;
+    PagedBatch b;
+    PagedGroups p;
+    const void *q;
+    void *out;
+    int64_t ld_q, ld_out;
+    const float *slopes;    // or null
+    const int32_t *prefix;  // or null
+    int32_t heads, window;
+    float scale, cap;
+    int32_t *status;
+};
 
 }  // namespace vh

@@ -347,6 +347,11 @@ void sync_status() {
     if (v & vh::kStatusF16Range) what = "an activation beyond the f16 range of the split-f16 matrix products";
     if (v & vh::kStatusFixRange)
         what += std::string(what.empty() ? "" : "; ") + "a fused-FFN term that is not finite or beyond +-2^18 (fixed-point range)";
+    std::string where;  // of the paged cache
+    if (v & vh::kStatusBadPage) where = "a page table entry outside the pool";
+    if (v & vh::kStatusBadBatch)
+        where += std::string(where.empty() ? "" : "; ") + "row_start, len or a position outside the batch, its page table or the rope table";
+    if (!where.empty()) throw Fail("paged cache: " + where + (what.empty() ? "" : "; value outside the device arithmetic's range: " + what));
     throw Fail("value outside the device arithmetic's range: " + what);
 }
 
@@ -3890,6 +3895,179 @@ int voxhip_quantize_act_dev(const float *d_x, int64_t n, int8_t *d_xq, float *d_
         HIPCHECK(launch_quant_act(d_x, n / 32, d_xq, d_xs, g.stream));
         HIPCHECK(hipStreamSynchronize(g.stream));
         return 1;
+    }, 0);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ paged cache
+namespace {
+// The library's device while a call launches: a caller's thread may have another one current.
+struct OnDevice {
+    int was = -1;
+    OnDevice() {
+        HIPCHECK(hipGetDevice(&was));
+        if (was != g.dev) HIPCHECK(hipSetDevice(g.dev));
+    }
+    ~OnDevice() {
+        if (was >= 0 && was != g.dev) (void)hipSetDevice(was);
+    }
+    OnDevice(const OnDevice &) = delete;
+    OnDevice &operator=(const OnDevice &) = delete;
+};
+
+constexpr int32_t kPagedMaxRows = 1 << 24, kPagedMaxSeqs = 1 << 20, kPagedMaxHeads = 1024;
+constexpr int64_t kPagedMaxKeys = int64_t(1) << 30;  // positions a page table may hold
+
+[[noreturn]] void paged_fail(const std::string &what) { throw Fail("paged cache: " + what); }
+void need(bool ok, const char *what) {
+    if (!ok) paged_fail(what);
+}
+// A device buffer of the call: there, aligned, and (VOXHIP_CHECK_HOST=1) device memory.
+void need_buf(const void *p, uintptr_t align, const char *what) {
+    if (!p) paged_fail(std::string(what) + " is missing");
+    if (reinterpret_cast<uintptr_t>(p) % align) paged_fail(std::string(what) + " is not aligned to " + std::to_string(align) + " bytes");
+    if (g.check_copies) check_copy_side(p, true, "paged cache", what);
+}
+size_t type_bytes(int32_t t) { return t == VOXHIP_F32 ? 4 : 2; }
+
+PagedKv paged_kv(const voxhip_paged_kv *kv) {
+    need(kv, "no cache");
+    need(kv->type == VOXHIP_F16 || kv->type == VOXHIP_BF16, "the cache is f16 or bf16");
+    need(kv->head_dim > 0 && kv->head_dim <= 128 && kv->head_dim % 8 == 0, "head_dim is a multiple of 8 up to 128");
+    need(kv->page_size >= 8 && kv->page_size <= 1024 && (kv->page_size & (kv->page_size - 1)) == 0, "page_size is a power of two from 8 to 1024");
+    need(kv->pages > 0, "no pages");
+    need(kv->kv_heads > 0 && kv->kv_heads <= kPagedMaxHeads, "kv_heads out of range");
+    need(kv->page_stride > 0 && kv->head_stride > 0 && kv->pos_stride >= kv->head_dim && kv->page_stride % 8 == 0 && kv->head_stride % 8 == 0 &&
+             kv->pos_stride % 8 == 0,
+         "strides are positive multiples of 8 elements, pos_stride at least head_dim");
+    // one page of one head, all heads and all pages lie apart: positions inside heads or heads inside positions, both inside a page
+    const int64_t in_head = int64_t(kv->page_size - 1) * kv->pos_stride + kv->head_dim, in_pos = int64_t(kv->kv_heads - 1) * kv->head_stride + kv->head_dim;
+    need(kv->kv_heads == 1 || kv->head_stride >= in_head || (kv->head_stride >= kv->head_dim && kv->pos_stride >= in_pos), "heads and positions of a page overlap");
+    need(kv->pages == 1 || kv->page_stride >= int64_t(kv->kv_heads - 1) * kv->head_stride + in_head, "pages overlap");
+    need(kv->page_stride <= INT64_MAX / 4 / kv->pages, "the pool is too large");
+    need_buf(kv->k, 16, "k");
+    need_buf(kv->v, 16, "v");
+    PagedKv c{};
+    c.k = kv->k; c.v = kv->v;
+    c.page_stride = kv->page_stride; c.head_stride = kv->head_stride; c.pos_stride = kv->pos_stride;
+    c.pages = kv->pages; c.kv_heads = kv->kv_heads; c.hd = kv->head_dim;
+    while ((1 << c.shift) < kv->page_size) ++c.shift;
+    return c;
+}
+// Whether there is anything to do.
+bool paged_batch(const voxhip_paged_batch *b, const PagedKv &c, PagedBatch *out) {
+    need(b, "no batch");
+    need(b->seqs >= 0 && b->seqs <= kPagedMaxSeqs && b->rows >= 0 && b->rows <= kPagedMaxRows, "sequences or rows out of range");
+    if (!b->seqs || !b->rows) return false;
+    need(b->max_rows > 0 && b->max_rows <= b->rows, "max_rows is not in 1..rows");
+    need(b->max_len > 0, "max_len is not positive");
+    need(b->page_ld > 0 && (b->page_ld << c.shift) <= kPagedMaxKeys, "page_ld out of range");
+    need(b->max_len <= (b->page_ld << c.shift), "max_len exceeds the page tables");
+    need_buf(b->row_start, 4, "row_start");
+    need_buf(b->len, 4, "len");
+    need_buf(b->pages, 4, "pages");
+    out->row_start = b->row_start; out->len = b->len; out->table = b->pages;
+    out->page_ld = b->page_ld; out->seqs = b->seqs; out->rows = b->rows;
+    return true;
+}
+void need_row_type(int32_t type, int32_t cache) {
+    need(type == VOXHIP_F32 || type == VOXHIP_F16 || type == VOXHIP_BF16, "rows are f32, f16 or bf16");
+    need((type == VOXHIP_BF16) == (cache == VOXHIP_BF16), "bf16 rows need a bf16 cache, f32 and f16 rows an f16 one");
+}
+void need_rows(const void *p, int64_t ld, int64_t cols, int32_t type, const char *what) {
+    need_buf(p, 16, what);
+    if (ld < cols || ld > (int64_t(1) << 32)) paged_fail(std::string(what) + ": the row stride is shorter than a row");
+    if (ld % 8) paged_fail(std::string(what) + ": the row stride is not a multiple of 8");
+}
+
+int kv_append(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r) {
+    AppendArgs a{};
+    a.c = paged_kv(kv);
+    need(r, "no rows");
+    need_row_type(r->type, kv->type);
+    need(r->heads > 0 && r->heads <= kPagedMaxHeads, "heads out of range");
+    need(r->heads % kv->kv_heads == 0, "heads is not a multiple of kv_heads");
+    if (!paged_batch(b, a.c, &a.b)) return 1;
+    const int64_t qd = int64_t(r->heads) * a.c.hd, kd = int64_t(a.c.kv_heads) * a.c.hd;
+    need_rows(r->qkv, r->ld_qkv, qd + 2 * kd, r->type, "qkv");
+    if (r->q) {
+        need_rows(r->q, r->ld_q, qd, r->type, "q");
+        const uintptr_t x = reinterpret_cast<uintptr_t>(r->qkv), y = reinterpret_cast<uintptr_t>(r->q);
+        const uintptr_t xe = x + uintptr_t(((int64_t(b->rows) - 1) * r->ld_qkv + qd + 2 * kd) * int64_t(type_bytes(r->type)));
+        const uintptr_t ye = y + uintptr_t(((int64_t(b->rows) - 1) * r->ld_q + qd) * int64_t(type_bytes(r->type)));
+        need(xe <= y || ye <= x, "q overlaps qkv");  // a lane reads values that another one rotates
+    }
+    if (r->q_norm) need_buf(r->q_norm, 16, "q_norm");
+    if (r->k_norm) need_buf(r->k_norm, 16, "k_norm");
+    need(!(r->q_norm || r->k_norm) || (std::isfinite(r->eps) && r->eps >= 0.f), "eps is negative or not finite");
+    if (r->rope) {
+        need_buf(r->rope, 16, "rope");
+        need(r->rope_len > 0, "rope_len is not positive");
+        need(r->rot_dim > 0 && r->rot_dim <= a.c.hd && r->rot_dim % 8 == 0, "rot_dim is a multiple of 8 up to head_dim");
+        a.rope = r->rope; a.rope_len = r->rope_len; a.rot = r->rot_dim; a.interleaved = r->interleaved != 0;
+    }
+    a.qkv = r->qkv; a.q = r->q; a.ld_qkv = r->ld_qkv; a.ld_q = r->ld_q;
+    a.qn = r->q_norm; a.kn = r->k_norm; a.eps = r->eps; a.heads = r->heads;
+    require_ok();
+    const OnDevice on;
+    vh::prof_stage("paged");
+    HIPCHECK(launch_kv_append(r->type, a, g.stream));
+    return 1;
+}
+
+int attn_paged(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_shared_prefix *p, const voxhip_attn_rows *r) {
+    PagedAttnArgs a{};
+    a.c = paged_kv(kv);
+    need(r, "no rows");
+    need_row_type(r->type, kv->type);
+    need(r->heads > 0 && r->heads <= kPagedMaxHeads, "heads out of range");
+    need(r->heads % kv->kv_heads == 0, "heads is not a multiple of kv_heads");
+    need(std::isfinite(r->scale), "scale is not finite");
+    need(std::isfinite(r->cap) && r->cap >= 0.f, "cap is negative or not finite");
+    need(r->window >= 0, "window is negative");
+    if (!paged_batch(b, a.c, &a.b)) return 1;
+    const int64_t qd = int64_t(r->heads) * a.c.hd;
+    need_rows(r->q, r->ld_q, qd, r->type, "q");
+    need_rows(r->out, r->ld_out, qd, r->type, "out");
+    if (r->out != r->q || r->ld_out != r->ld_q) {  // in place, or apart
+        const uintptr_t x = reinterpret_cast<uintptr_t>(r->q), y = reinterpret_cast<uintptr_t>(r->out);
+        const int64_t tb = int64_t(type_bytes(r->type)), last = int64_t(b->rows) - 1;
+        need(x + uintptr_t((last * r->ld_q + qd) * tb) <= y || y + uintptr_t((last * r->ld_out + qd) * tb) <= x, "out overlaps q partly");
+    }
+    if (r->slopes) need_buf(r->slopes, 4, "slopes");
+    if (r->prefix) need_buf(r->prefix, 4, "prefix");
+    if (p) {
+        need(p->groups >= 0 && p->groups <= b->seqs, "more groups than sequences");
+        if (p->groups) {
+            need(p->max_len >= 0 && p->max_len <= b->max_len, "the shared max_len is not in 0..max_len");
+            need_buf(p->seq_start, 4, "seq_start");
+            need_buf(p->len, 4, "the groups' len");
+            a.p.seq_start = p->seq_start; a.p.len = p->len; a.p.groups = p->groups;
+        }
+    }
+    a.q = r->q; a.out = r->out; a.ld_q = r->ld_q; a.ld_out = r->ld_out;
+    a.slopes = r->slopes; a.prefix = r->prefix; a.heads = r->heads; a.window = r->window;
+    a.scale = r->scale; a.cap = r->cap;
+    require_ok();
+    const OnDevice on;
+    vh::prof_stage("paged");
+    HIPCHECK(launch_paged_attn(r->type, a, g.stream));
+    return 1;
+}
+}  // namespace
+
+extern "C" {
+int voxhip_kv_append_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r) {
+    return guard_int([&] { return kv_append(kv, b, r); }, 0);
+}
+int voxhip_attn_paged_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_attn_rows *r) {
+    return guard_int([&] { return attn_paged(kv, b, nullptr, r); }, 0);
+}
+int voxhip_attn_shared_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_shared_prefix *p, const voxhip_attn_rows *r) {
+    return guard_int([&] {
+        if (!p) paged_fail("no shared prefixes");
+        return attn_paged(kv, b, p, r);
     }, 0);
 }
 

@@ -138,6 +138,32 @@ class CodecDesc(C.Structure):
                 ("final_act", CodecSnake), ("final_conv", CodecConv)]
 
 
+class PagedKv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int32) for n in ("type", "pages", "page_size", "kv_heads", "head_dim")] + \
+               [(n, C.c_int64) for n in ("page_stride", "head_stride", "pos_stride")]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("seqs", "rows", "max_rows", "max_len")] + \
+               [(n, C.c_void_p) for n in ("row_start", "len", "pages")] + [("page_ld", C.c_int64)]
+
+
+class AppendRows(C.Structure):
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("qkv", C.c_void_p), ("ld_qkv", C.c_int64), ("q", C.c_void_p),
+                ("ld_q", C.c_int64), ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("eps", C.c_float), ("rope", C.c_void_p)] + \
+               [(n, C.c_int32) for n in ("rope_len", "rot_dim", "interleaved")]
+
+
+class AttnRows(C.Structure):
+    _fields_ = [("type", C.c_int32), ("heads", C.c_int32), ("q", C.c_void_p), ("ld_q", C.c_int64), ("out", C.c_void_p),
+                ("ld_out", C.c_int64), ("scale", C.c_float), ("cap", C.c_float), ("slopes", C.c_void_p), ("prefix", C.c_void_p),
+                ("window", C.c_int32)]
+
+
+class SharedPrefix(C.Structure):
+    _fields_ = [("groups", C.c_int32), ("max_len", C.c_int32), ("seq_start", C.c_void_p), ("len", C.c_void_p)]
+
+
 KERNEL_CLASSES = ("qkv_gemv", "o_gemv", "gateup_gemv", "down_gemv", "head_gemv", "attention", "attn_combine", "qk_post", "sampler",
                   "ffn", "acc_fold", "quant_rows")
 
@@ -216,6 +242,9 @@ SIGNATURES = {
     "voxhip_quantize_q8_dev": (_I, [_P, _I64, _I64, _P, _P]),
     "voxhip_quantize_q4_dev": (_I, [_P, _I64, _I64, _P, _P]),
     "voxhip_quantize_act_dev": (_I, [_P, _I64, _P, _P]),
+    "voxhip_kv_append_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(AppendRows)]),
+    "voxhip_attn_paged_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(AttnRows)]),
+    "voxhip_attn_shared_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(SharedPrefix), C.POINTER(AttnRows)]),
     "voxhip_bench_decode": (_I, [_I, _I, _I64, _P, _I, C.POINTER(SampleCfg), _P, _I, _I, C.POINTER(BenchResult)]),
     "voxhip_bench_decode_steps": (_I, [_I, _P, _P, _I64, _P, _I, _P, _P, _I, _I, C.POINTER(BenchResult)]),
     "voxhip_bench_gemv_q8": (_I, [_I64, _I64, _I, _I, _I, C.POINTER(C.c_double)]),
@@ -828,6 +857,53 @@ def quantize_act_dev(x):
     finally:
         for b in (dx, dq, ds):
             b.free()
+
+
+# ---------------------------------------------------------------- paged cache (device buffers: anything with .ptr)
+def _ptr(b):
+    return None if b is None else b.ptr
+
+
+def paged_kv(k, v, wtype, pages, page_size, kv_heads, head_dim, page_stride=None, head_stride=None, pos_stride=None):
+    """One layer's pool of pages: [pages][kv_heads][page_size][head_dim] unless strides (in elements) say otherwise."""
+    pos = head_dim if pos_stride is None else pos_stride
+    head = page_size * pos if head_stride is None else head_stride
+    page = kv_heads * head if page_stride is None else page_stride
+    return PagedKv(_ptr(k), _ptr(v), wtype, pages, page_size, kv_heads, head_dim, page, head, pos)
+
+
+def paged_batch(seqs, rows, max_rows, max_len, row_start, lens, pages, page_ld):
+    """A ragged batch: row_start [seqs + 1], lens [seqs], pages [seqs][page_ld] (int32 device buffers)."""
+    return PagedBatch(seqs, rows, max_rows, max_len, _ptr(row_start), _ptr(lens), _ptr(pages), page_ld)
+
+
+def append_rows(wtype, heads, qkv, ld_qkv, q=None, ld_q=0, q_norm=None, k_norm=None, eps=1e-6, rope=None, rope_len=0, rot_dim=0,
+                interleaved=False):
+    return AppendRows(wtype, heads, _ptr(qkv), ld_qkv, _ptr(q), ld_q, _ptr(q_norm), _ptr(k_norm), eps, _ptr(rope), rope_len, rot_dim,
+                      int(bool(interleaved)))
+
+
+def attn_rows(wtype, heads, q, ld_q, out, ld_out, scale, cap=0.0, slopes=None, prefix=None, window=0):
+    return AttnRows(wtype, heads, _ptr(q), ld_q, _ptr(out), ld_out, scale, cap, _ptr(slopes), _ptr(prefix), window)
+
+
+def shared_prefix(groups, max_len, seq_start, lens):
+    return SharedPrefix(groups, max_len, _ptr(seq_start), _ptr(lens))
+
+
+def kv_append_dev(kv, batch, rows):
+    """Turned and normed q of the batch's rows, their k and v into the pages (asynchronous on the library's stream)."""
+    _check(lib().voxhip_kv_append_dev(C.byref(kv), C.byref(batch), C.byref(rows)), "kv_append_dev")
+
+
+def attn_paged_dev(kv, batch, rows):
+    """Attention of the batch's rows on the pages (asynchronous on the library's stream)."""
+    _check(lib().voxhip_attn_paged_dev(C.byref(kv), C.byref(batch), C.byref(rows)), "attn_paged_dev")
+
+
+def attn_shared_dev(kv, batch, shared, rows):
+    """attn_paged_dev with the shared keys of groups of sequences read once for all of a group's rows."""
+    _check(lib().voxhip_attn_shared_dev(C.byref(kv), C.byref(batch), C.byref(shared), C.byref(rows)), "attn_shared_dev")
 
 
 def bench_decode(xfmr, seq, pos0, d_x, head, cfg, d_token, warmup, steps):
