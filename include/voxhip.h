@@ -447,7 +447,7 @@ int voxhip_quantize_act_dev(const float *d_x, int64_t n, int8_t *d_xq, float *d_
  * serialise; the library's own workspace is shared by them all.
  *
  * Device contents are not checked by the host. A table entry that names no page of the pool, or row_start / len beyond the
- * buffers, touches nothing outside them: those keys are left out, those rows not written or of no meaning, and the next
+ * buffers, touches nothing outside them: those keys are read as zeros, those rows not written or of no meaning, and the next
  * voxhip_sync (or synchronous call) fails. */
 /* One layer's pool: element d of kv head h at position p of a sequence lies at
  * page * page_stride + h * head_stride + (p % page_size) * pos_stride + d elements of k (and of v), page = the sequence's

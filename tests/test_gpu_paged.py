@@ -483,3 +483,17 @@ def test_bad_tables_are_reported(hip):
         assert torch.equal(r.attend(q), before)
     finally:
         r.free()
+
+
+def test_range_of_f32_queries(hip):
+    """A query beyond the f16 range, which the split of f32 rows cannot hold, is reported as elsewhere in the library."""
+    b = Batch([1], [20], F32, 2, 1, 64, 16, seed=2)
+    q = b.normal(1, 128)
+    q[0, 5] = 7e4
+    r = Run(hip, b)
+    try:
+        with pytest.raises(hip.VoxHipError, match="f16 range"):
+            r.attend(q)
+        r.attend(b.normal(1, 128))
+    finally:
+        r.free()

@@ -1,4 +1,6 @@
 // Launchers of the paged-cache kernels.
+#include <algorithm>
+
 #include "vh_launch.hpp"
 #include "vh_paged.hpp"
 
@@ -30,12 +32,71 @@ hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     });
 }
 
-hipError_t launch_paged_attn(int type, PagedAttnArgs a, hipStream_t s) {
-    const int64_t grid = int64_t(a.b.rows) * a.heads;
-    if (a.c.hd <= 0 || a.c.hd > 128 || a.b.rows <= 0 || a.b.seqs <= 0 || grid > INT32_MAX) return hipErrorInvalidValue;
+// Tiles of 16, 32 or 128 query rows by the most that a segment can have; runs so that the launch has a few blocks for each of
+// the 256 CUs, of no fewer than kLeastKeys keys.
+PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_len, int32_t max_shared) {
+    constexpr int32_t kLeastKeys = 256, kMostSplits = 32, kBlocks = 512;
+    const int32_t G = a.c.kv_heads, group = a.heads / G;
+    auto tile_for = [](int64_t q) { return q <= 16 ? 16 : q <= 32 ? 32 : 128; };
+    auto splits_for = [&](int64_t tiles, int32_t keys) {
+        const int64_t want = (kBlocks + tiles * G - 1) / (tiles * G), most = (int64_t(keys) + kLeastKeys - 1) / kLeastKeys;
+        return int32_t(std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits})));
+    };
+    PagedPlan p{};
+    p.gleast = p.sleast = kLeastKeys;
+    const int64_t q = int64_t(a.b.rows) * group;
+    p.stile = tile_for(int64_t(max_rows) * group);
+    p.direct = int64_t(max_rows) * group <= p.stile;
+    p.stiles = int32_t(p.direct ? a.b.seqs : std::min<int64_t>(q / p.stile + a.b.seqs, INT32_MAX));
+    p.ssplits = splits_for(p.stiles, max_len);
+    if (a.p.groups) {
+        p.gtile = tile_for(q);
+        p.gtiles = int32_t(q / p.gtile + a.p.groups);
+        p.gsplits = splits_for(std::max<int64_t>(1, q / p.gtile), std::max(max_shared, 1));
+    }
+    p.slots = p.gsplits + p.ssplits;
+    p.ws_floats = p.gsplits || p.ssplits > 1 ? int64_t(a.b.rows) * a.heads * p.slots * (2 + a.c.hd) : 0;
+    return p;
+}
+
+namespace {
+template <class T, class C, int HDP, int NQ, int WQ, bool GROUPS>
+hipError_t attn_launch(const PagedAttnArgs &a, int32_t tiles, int32_t splits, int32_t least, bool direct, hipStream_t s) {
+    constexpr size_t pitch = HDP <= 64 ? 128 : 256, stages = size_t(4 / WQ) * 2 * 2 * (WQ == 4 ? 64 : 32) * pitch;
+    constexpr size_t join = WQ == 4 ? 0 : (size_t(2) * 4 * NQ + size_t(4) * NQ * (HDP + 4)) * 4, smem = stages > join ? stages : join;
+    const int64_t grid = int64_t(tiles) * splits * a.c.kv_heads;
+    if (grid > INT32_MAX) return hipErrorInvalidValue;
+    auto *k = k_paged_attn<T, C, HDP, NQ, WQ, GROUPS>;
+    if (const hipError_t e = ensure_smem(reinterpret_cast<const void *>(k), smem); e != hipSuccess) return e;
+    return launch(k, dim3(unsigned(grid)), dim3(256), smem, s, a, tiles, splits, least, int32_t(direct));
+}
+template <class T, class C, int HDP>
+hipError_t attn_of(const PagedAttnArgs &a, const PagedPlan &p, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    if (p.gtile == 16) e = attn_launch<T, C, HDP, 16, 1, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
+    else if (p.gtile == 32) e = attn_launch<T, C, HDP, 32, 1, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
+    else if (p.gtile) e = attn_launch<T, C, HDP, 32, 4, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
+    if (e != hipSuccess) return e;
+    if (p.stile == 16) return attn_launch<T, C, HDP, 16, 1, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
+    if (p.stile == 32) return attn_launch<T, C, HDP, 32, 1, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
+    return attn_launch<T, C, HDP, 32, 4, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
+}
+}  // namespace
+
+hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &p, float *ws, hipStream_t s) {
+    if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0 || (p.ws_floats && !ws)) return hipErrorInvalidValue;
+    const int64_t join = int64_t(a.b.rows) * ((a.heads + 7) / 8);
+    if (join > INT32_MAX) return hipErrorInvalidValue;
     a.status = status_word();
+    a.slots = p.slots; a.gsplits = p.gsplits; a.ssplits = p.ssplits; a.gleast = p.gleast; a.sleast = p.sleast;
+    a.po = ws;  // 16-byte aligned rows first
+    a.ml = ws ? ws + int64_t(a.b.rows) * a.heads * p.slots * a.c.hd : nullptr;
     return by_type(type, [&](auto t, auto c) {
-        return launch(k_paged_attn_rows<decltype(t), decltype(c)>, dim3(unsigned(grid)), dim3(256), 0, s, a);
+        using T = decltype(t);
+        using C = decltype(c);
+        const hipError_t e = a.c.hd <= 64 ? attn_of<T, C, 64>(a, p, s) : a.c.hd <= 96 ? attn_of<T, C, 96>(a, p, s) : attn_of<T, C, 128>(a, p, s);
+        if (e != hipSuccess || !p.ws_floats) return e;
+        return launch(k_paged_join<T>, dim3(unsigned(join)), dim3(256), 0, s, a);
     });
 }
 

@@ -1,6 +1,8 @@
 // vh_paged.hpp — a key/value cache in pages: the append of a step's rows with their rotation, and the attention that
 // reads it (gfx950, wave64).
 #pragma once
+#include <type_traits>
+
 #include "vh_common.hpp"
 #include "vh_paged_index.hpp"
 #include "vh_types.hpp"
@@ -106,62 +108,570 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     store4(dst, x);
 }
 
-// One (row, head) per block of 4 waves: wave w takes keys begin + w, + 4, ..., lane l dims l and l + 64, an online softmax
-// per wave, the waves merged through LDS.
-template <class T, class C>
-__global__ __launch_bounds__(256) void k_paged_attn_rows(PagedAttnArgs a) {
-    const int row = int(blockIdx.x) / a.heads, h = int(blockIdx.x) % a.heads;
-    const int hd = a.c.hd, g = h / (a.heads / a.c.kv_heads), lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// ------------------------------------------------------------------ attention
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+// Matrix products of the cache's type: c += a b, columns of b in the lanes' low bits, the K elements of a lane neighbours.
+template <class C>
+struct Mx;
+template <>
+struct Mx<_Float16> {
+    typedef f16x8 v8;
+    static constexpr uint16_t kExp = 0x7C00, kOne = 0x3C00;
+    static VH_DEV f32x16 mm(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static VH_DEV f32x4 mm(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mx<__bf16> {
+    typedef bf16x8 v8;
+    static constexpr uint16_t kExp = 0x7F80, kOne = 0x3F80;
+    static VH_DEV f32x16 mm(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static VH_DEV f32x4 mm(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// What lanes without a key (behind a sequence's last, past head_dim) read instead.
+static __device__ __align__(16) uint32_t kZero16[4];
+
+// 16 bytes per lane from its own address to LDS lds + 16 lane; as dma_b128, the waits are the caller's.
+VH_DEV void dma_lane16(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+// Every LDS read of this wave has returned, then the block's barrier.
+VH_DEV void read_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+VH_DEV void block_barrier() { asm volatile("s_barrier" ::: "memory"); }
+
+VH_DEV float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Maximum, sum over the lanes that hold one query row (64 / NQ, NQ apart); every one of them gets it.
+template <int NQ>
+VH_DEV float rows_max(float v) {
+    if (NQ == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int NQ>
+VH_DEV float rows_sum(float v) {
+    if (NQ == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// tanh to about 2^-23 of its value: odd polynomial (Taylor, to x^11) below 0.3, (1 - t) / (1 + t) with t = 2^(-2 |x| log2 e)
+// above, where 1 - t cancels little.
+VH_DEV float tanh_f(float x) {
+    const float a = fabsf(x), x2 = x * x;
+    const float t = exp2_fast(-2.8853900817779268f * a);
+    const float big = copysignf((1.f - t) / (1.f + t), x);
+    float p = fmaf(x2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    p = fmaf(x2, p, -17.0f / 315.0f);
+    p = fmaf(x2, p, 2.0f / 15.0f);
+    p = fmaf(x2, p, -1.0f / 3.0f);
+    return a < 0.3f ? fmaf(x * x2, p, x) : big;
+}
+
+// The segment (of n, with rows_of(i) rows each) and the tile in it of the launch's tile t: 64 segments at a time.
+template <class F>
+VH_DEV bool find_tile(int32_t n, int32_t t, int32_t group, int32_t tile, F rows_of, int32_t *seg, int32_t *local) {
+    const int lane = threadIdx.x & 63;
+    for (int32_t base = 0; base < n; base += 64) {
+        const int32_t mine = base + lane < n ? tiles_of(rows_of(base + lane), group, tile) : 0;
+        int32_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int32_t up = __shfl_up(sum, o, 64);
+            sum += lane >= o ? up : 0;
+        }
+        const uint64_t past = __ballot(sum > t);
+        if (past) {
+            const int l = __ffsll(static_cast<unsigned long long>(past)) - 1;
+            *seg = base + l;
+            *local = t - (__builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(mine, l));
+            return true;
+        }
+        t -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+// Softmax attention of a tile of query rows over a run of keys, on the matrix cores, transposed: S^T = K Q^T has a query row's
+// scores in the registers of one lane (two with 32 x 32 products, four with 16 x 16), so a row's maximum is a few register
+// maxima and one or two lane swaps, the rescale of O^T is by a lane's own factor, and P^T is already the operand that O^T +=
+// V^T P^T wants: the K index of that product is the order in which S^T's rows lie in registers, and V^T's operand is read in the
+// same order by the transposing LDS read (4 keys at a time). Keys and values come to LDS by DMA, in 16-byte pieces at
+// piece ^ f(key), so that neither the row-wise reads of K nor the 4 x 16 blocks of V meet in a bank.
+//
+// NQ query rows per wave, WQ waves beside each other on the same keys, the other 4 / WQ on other keys (tiles of KW keys each,
+// every 4 / WQ-th), joined through LDS at the end. WQ = 4 (128 rows, prompts and tall prefixes): keys are read from LDS for
+// 128 rows at once, bound by the products and the exponentials beside them. WQ = 1 (16 or 32 rows, steps): every wave streams its
+// own keys, no barrier in the loop, bound by the bytes.
+//
+// f32 rows: q and the weights as two f16 halves, both multiplied (exact products, to about 2^-22). f16 / bf16 rows: the
+// weights are rounded to the cache's type, half a step each; sums, maxima and outputs stay in 32 bits. Weights are
+// 2^(s - m + kUp) with m within 2^kLag of the running maximum: the running maximum only moves (and O^T is only rescaled) when a
+// score passes it by more than kLag, and kUp keeps small f16 weights out of the subnormals.
+template <class T, class C, int HDP, int NQ, int WQ, bool GROUPS>
+__global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnArgs a, int32_t tiles, int32_t splits, int32_t least, int32_t direct) {
+    typedef typename Mx<C>::v8 v8;
+    typedef typename std::conditional<NQ == 32, f32x16, f32x4>::type acc;
+    constexpr bool kSplit = std::is_same<T, float>::value;
+    constexpr int WK = 4 / WQ, KW = WQ == 4 ? 64 : 32, TILE = NQ * WQ;
+    constexpr int PITCH = HDP <= 64 ? 128 : 256, CPR = PITCH / 16, R = 64 / CPR;  // bytes of a key in LDS, its pieces, keys a DMA
+    constexpr int KB = KW * PITCH, STAGE = 2 * KB;                                // K then V of a tile
+    constexpr int NI = KW / R / WQ;                                               // DMAs of K (and of V) a wave and tile
+    constexpr int KD = NQ == 32 ? 16 : 32;                                        // K of one product
+    constexpr int SUB = NQ, NSUB = KW / SUB, AV = NQ == 32 ? 16 : 4;              // keys of one S^T product, values a lane
+    constexpr int ND = HDP / NQ;                                                  // O^T products
+    constexpr int NC = KW / KD;                                                   // P^T operands
+    constexpr float kUp = std::is_same<C, __bf16>::value ? 0.f : 6.f, kLag = 8.f;
+    static_assert(NI >= 1 && (NI % 2 == 0 || R == 8), "the swizzle's parity is the DMA's");
+    extern __shared__ __align__(16) uint8_t smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    const int wq = wave % WQ, wk = wave / WQ, col = lane % NQ, lh = lane / NQ;  // lh: which rows of a product this lane holds
+    const int G = a.c.kv_heads, group = a.heads / G, hd = a.c.hd;
+    const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((lds_void *)smem));
+    // kv heads are the fastest index: blocks of one kv head (and its keys) meet in few XCDs' L2
+    int id = blockIdx.x;
+    const int g = id % G;
+    id /= G;
+    const int split = id % splits;
+    int32_t t = id / splits, seg_id = t, local = 0;
+    Segment seg;
+    if constexpr (GROUPS) {
+        if (!find_tile(a.p.groups, t, group, TILE, [&](int32_t i) { return group_segment(a.b, a.p, a.c.shift, i).rows; }, &seg_id, &local)) return;
+        seg = group_segment(a.b, a.p, a.c.shift, seg_id);
+    } else {
+        t = tiles - 1 - t;  // the last tiles of a prompt see the most keys: first
+        seg_id = t;
+        if (!direct && !find_tile(a.b.seqs, t, group, TILE,
+                                  [&](int32_t i) {
+                                      const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
+                                      return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
+                                  },
+                                  &seg_id, &local))
+            return;
+        seg = seq_segment(a.b, a.p, a.c.shift, seg_id);
+    }
+    const int32_t qrows = seg.rows * group;
+    raise_status(a.status, threadIdx.x == 0 && (!seg.ok || (direct && qrows > TILE)), kStatusBadBatch);
+    if (local * TILE >= qrows) return;
+    const Runs runs = runs_of(seg.key0, seg.key1, splits, least);
+    // a row whose keys are one run is written here, otherwise its parts are joined by k_paged_join
+    bool whole = false;
+    int32_t slot0 = 0;
+    if constexpr (!GROUPS) {
+        const int32_t grp = group_of(a.p, seg_id);
+        const Runs gr = grp >= 0 ? runs_of(0, clamp_i32(a.p.len[grp], 0, a.b.page_ld << a.c.shift), a.gsplits, a.gleast) : Runs{0, 0, 0};
+        whole = gr.count == 0 && runs.count <= 1;
+        slot0 = a.gsplits;
+    }
+    if (split >= runs.count && !(whole && split == 0)) return;
+    const Span run = runs.count ? run_at(runs, seg.key0, seg.key1, split) : Span{0, 0};
+
+    // this lane's query row
+    const int32_t u = local * TILE + wq * NQ + col;
+    const bool valid = u < qrows;
+    const int32_t tok = valid ? u / group : 0, row = seg.row0 + tok, head = g * group + (valid ? u - tok * group : 0);
+    int32_t seq = seg.seq0;
+    if constexpr (GROUPS) {  // the sequence that holds the row: by the guess of one row each, or halving
+        seq = min(seg.seq0 + tok, seg.seq1 - 1);
+        if (!(a.b.row_start[seq] <= row && row < a.b.row_start[seq + 1])) {
+            int32_t lo = seg.seq0, hi = seg.seq1;  // the last s with row_start[s] <= row
+            while (hi - lo > 1) {
+                const int32_t mid = (lo + hi) >> 1;
+                if (a.b.row_start[mid] <= row) lo = mid;
+                else hi = mid;
+            }
+            seq = lo;
+        }
+    }
+    const SeqRows sr = seq_rows(a.b, a.c.shift, seq);
+    const int32_t pos = sr.len - sr.n + (row - sr.first);
+    Span see = visible(pos, sr.len, a.prefix ? a.prefix[seq] : 0, a.window);
+    see.begin = max(see.begin, run.begin);
+    see.end = valid ? min(see.end, run.end) : 0;
+    if (see.begin >= see.end) see = Span{0, 0};
+    const uint32_t see_n = uint32_t(see.end - see.begin);
+    // of the wave's rows: the keys that any sees, and those that all see
+    int32_t lo_any = see_n ? see.begin : INT32_MAX, hi_any = see.end, lo_all = valid ? (see_n ? see.begin : INT32_MAX) : 0,
+            hi_all = valid ? see.end : INT32_MAX;
+#pragma unroll
+    for (int o = 1; o < NQ; o <<= 1) {
+        lo_any = min(lo_any, __shfl_xor(lo_any, o, 64));
+        hi_any = max(hi_any, __shfl_xor(hi_any, o, 64));
+        lo_all = max(lo_all, __shfl_xor(lo_all, o, 64));
+        hi_all = min(hi_all, __shfl_xor(hi_all, o, 64));
+    }
+    lo_any = __builtin_amdgcn_readfirstlane(lo_any);
+    hi_any = __builtin_amdgcn_readfirstlane(hi_any);
+    lo_all = __builtin_amdgcn_readfirstlane(lo_all);
+    hi_all = __builtin_amdgcn_readfirstlane(hi_all);
+    // the block's keys: of a sequence's tile from its first and last row, of a group's the run
+    int32_t kb = run.begin, ke = run.end;
+    if constexpr (!GROUPS) {
+        const int32_t t0 = local * TILE / group, t1 = min(local * TILE + TILE, qrows) - 1, pf = a.prefix ? a.prefix[seg_id] : 0;
+        const int32_t p0 = sr.len - sr.n + t0, p1 = sr.len - sr.n + t1 / group;
+        kb = max(kb, visible(p0, sr.len, pf, a.window).begin);
+        ke = min(ke, visible(p1, sr.len, pf, a.window).end);
+    }
+    kb = __builtin_amdgcn_readfirstlane(kb & ~(KW * WK - 1));
+    ke = __builtin_amdgcn_readfirstlane(ke);
+
+    // queries as the second operand of S^T: column col, K elements 8 lh .. of every product. A negative scale turns them
+    // around, so that the largest product is the largest score.
+    constexpr int NK = HDP / KD;
+    v8 qh[NK], ql[kSplit ? NK : 1];
+    {
+        const T *qr = static_cast<const T *>(a.q) + int64_t(row) * a.ld_q + int64_t(head) * hd;
+        const float sign = a.scale < 0.f ? -1.f : 1.f;
+        bool bad = false;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            const int d = KD * c + 8 * lh;
+            const bool in = valid && d < hd;
+            if constexpr (kSplit) {
+                f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
+                if (in) {
+                    x0 = *reinterpret_cast<const f32x4 *>(qr + d);
+                    x1 = *reinterpret_cast<const f32x4 *>(qr + d + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 hi, lo;
+                    bad |= split_f16(sign * (e < 4 ? x0[e] : x1[e - 4]), hi, lo);
+                    qh[c][e] = hi;
+                    ql[c][e] = lo;
+                }
+            } else {
+                u32x4 x = {0u, 0u, 0u, 0u};
+                if (in) x = *reinterpret_cast<const u32x4 *>(qr + d);
+                const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+                qh[c] = __builtin_bit_cast(v8, x ^ u32x4{flip, flip, flip, flip});
+            }
+        }
+        raise_status(a.status, bad, kStatusF16Range);
+    }
+    constexpr float kLog2e = 1.44269504088896341f;
+    const bool capped = a.cap > 0.f, biased = a.slopes != nullptr;
+    const float sc = fabsf(a.scale) * (capped ? 1.f / a.cap : kLog2e), cap2 = a.cap * kLog2e;
+    const float slope = biased ? a.slopes[head] * kLog2e : 0.f;
+
+    // DMA: this lane's key of R and piece of CPR, by the DMA's parity where the swizzle needs it
+    const int rin = lane / CPR, piece = lane % CPR;
+    int64_t voff[2];
+    bool vin[2];
+#pragma unroll
+    for (int par = 0; par < 2; ++par) {
+        const int p = PITCH == 256 ? piece ^ (((4 * par + rin) & 7) << 1) : piece ^ (((rin >> 1) & 3) << 1);
+        voff[par] = (int64_t(rin) * a.c.pos_stride + 8 * p) * 2;
+        vin[par] = 8 * p < hd;
+    }
+    const int32_t *tab = a.b.table + int64_t(seg.seq0) * a.b.page_ld;
+    const int32_t last_page = run.end > run.begin ? (run.end - 1) >> a.c.shift : 0, first_page = run.begin >> a.c.shift;
+    int32_t pg = -1, pbase = -64;  // lane l: the page of table entry pbase + l
+    bool bad_page = false;
+    auto issue = [&](int32_t kt, uint32_t buf) {
+        const int32_t i0 = max(kt >> a.c.shift, first_page), i1 = min((kt + KW - 1) >> a.c.shift, last_page);
+        if (i0 < pbase || i1 >= pbase + 64) {
+            pbase = i0;
+            const int32_t i = i0 + lane;
+            const bool in = i <= last_page;
+            const int32_t e = in ? tab[i] : -1;
+            pg = uint32_t(e) < uint32_t(a.c.pages) ? e : -1;
+            bad_page |= in && pg < 0;
+        }
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int i = wq * NI + n, par = n & 1;
+            const int32_t key = kt + R * i, pi = min(max(key >> a.c.shift, i0), i1);
+            const int32_t page = __builtin_amdgcn_readlane(pg, (pi - pbase) & 63);
+            const int64_t at = (int64_t(page) * a.c.page_stride + int64_t(g) * a.c.head_stride +
+                                int64_t(key & ((1 << a.c.shift) - 1)) * a.c.pos_stride) * 2 + voff[par];
+            const bool in = page >= 0 && vin[par] && key + rin >= run.begin && key + rin < run.end;
+            const void *zero = kZero16;
+            dma_lane16(in ? static_cast<const uint8_t *>(a.c.k) + at : zero, buf + i * 1024);
+            dma_lane16(in ? static_cast<const uint8_t *>(a.c.v) + at : zero, buf + KB + i * 1024);
+        }
+    };
+
+    acc o[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < AV; ++i) o[d][i] = 0.f;
+    float m = -INFINITY, l = 0.f;  // m: the running maximum in log2 units; l: this lane's share of the sum
+    // LDS addresses: K operand, key col (+ NQ j), piece (KD / 8) c + lh; V^T operand, key 4 (lane / 16 or lh) + lane / 4 % 4,
+    // dims 4 (lane % 4) of 16 (and the upper 16 of 32 for odd lane / 16)
+    const int ksw = PITCH == 256 ? (col & 7) << 1 : ((col >> 1) & 3) << 1;
+    const int vi = lane & 15, vkey = (NQ == 32 ? 4 * lh : 4 * (lane >> 4)) + (vi >> 2), vd = (NQ == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((vi & 3) >> 1);
+    const int vsw = PITCH == 256 ? (vkey & 7) << 1 : ((vkey >> 1) & 3) << 1;
+    const uint32_t stream = uint32_t(wk) * 2 * STAGE;
+    // value i of S^T product j: its key in the tile
+    auto key_in = [&](int j, int i) { return SUB * j + (NQ == 32 ? (i & 3) + 8 * (i >> 2) + 4 * lh : i + 4 * lh); };
+
+    const int32_t k_first = kb + wk * KW;
+    const bool some = ke > kb;
+    if (some && k_first < ke) issue(k_first, lds0 + stream);
+    int stage = 0;
+    for (int32_t kt = k_first; kt < ke; kt += KW * WK, stage ^= 1) {
+        const bool more = kt + KW * WK < ke;
+        if constexpr (WQ == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other stage's reads are done
+        if (more) issue(kt + KW * WK, lds0 + stream + (stage ^ 1) * STAGE);
+        if (more) wait_step<2 * NI>();
+        else wait_step<0>();
+        if constexpr (WQ > 1) block_barrier();
+        const uint8_t *Ks = smem + stream + stage * STAGE, *Vs = Ks + KB;
+        if (lo_any < kt + KW && hi_any > kt) {
+            const bool full = lo_all <= kt && hi_all >= kt + KW;
+            acc s[NSUB];
+#pragma unroll
+            for (int j = 0; j < NSUB; ++j) {
+#pragma unroll
+                for (int i = 0; i < AV; ++i) s[j][i] = 0.f;
+#pragma unroll
+                for (int c = 0; c < NK; ++c) {
+                    const v8 k = *reinterpret_cast<const v8 *>(Ks + (SUB * j + col) * PITCH + (((KD / 8 * c + lh) ^ ksw) << 4));
+                    s[j] = Mx<C>::mm(k, qh[c], s[j]);
+                    if constexpr (kSplit) s[j] = Mx<C>::mm(k, ql[c], s[j]);
+                }
+            }
+            float unit = sc;  // of s, in log2 units
+            if (capped || biased || sc == 0.f) {  // (a scale of zero times a masked score is no number)
+#pragma unroll
+                for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+                    for (int i = 0; i < AV; ++i) {
+                        float z = s[j][i] * sc;
+                        if (capped) z = cap2 * tanh_f(z);
+                        if (biased) z -= slope * fabsf(float(pos - kt - key_in(j, i)));
+                        s[j][i] = z;
+                    }
+                unit = 1.f;
+            }
+            if (!full) {
+#pragma unroll
+                for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+                    for (int i = 0; i < AV; ++i)
+                        s[j][i] = uint32_t(kt + key_in(j, i) - see.begin) < see_n ? s[j][i] : -INFINITY;
+            }
+            float mx = s[0][0];
+#pragma unroll
+            for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+                for (int i = 0; i < AV; ++i) mx = fmaxf(mx, s[j][i]);
+            mx = rows_max<NQ>(mx);
+            mx *= unit;
+            if (__any(mx > m + kLag || (m == -INFINITY && mx != m))) {
+                const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.f : exp2_fast(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int i = 0; i < AV; ++i) o[d][i] *= f;
+            }
+            const float add = m == -INFINITY ? 0.f : kUp - m;
+            // P^T operand c, and its share of the sum
+            auto weights = [&](int c, v8 &ph, v8 &pl) {
+                float p[8], sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    // 32 x 32: 8 neighbouring registers; 16 x 16: the 4 of two products
+                    const float x = NQ == 32 ? s[c / 2][(8 * c + e) & 15] : s[2 * c + e / 4][e & 3];
+                    p[e] = exp2_fast(fmaf(x, unit, add));
+                    sum += p[e];
+                }
+                if constexpr (kSplit) {
+                    u32x4 h4, l4;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        uint32_t hi, lo;
+                        split_f16x2(p[2 * e], p[2 * e + 1], hi, lo);
+                        h4[e] = hi;
+                        l4[e] = lo;
+                    }
+                    ph = __builtin_bit_cast(v8, h4);
+                    pl = __builtin_bit_cast(v8, l4);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) ph[e] = C(p[e]);
+                }
+                return sum;
+            };
+            auto v_at = [&](int c, int d) {
+                // keys KD c + (4 neighbours, then 4 neighbours 8 or 16 on), dims NQ d ..
+                const uint8_t *at = Vs + (KD * c + vkey) * PITCH + (((NQ / 8 * d + vd) ^ vsw) << 4) + (vi & 1) * 8;
+                union {
+                    s16x4 half[2];
+                    v8 whole;
+                } r;
+                r.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
+                r.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + (NQ == 32 ? 8 : 16) * PITCH));
+                return r.whole;
+            };
+            // A value that is not finite may stand at a key that only some rows see: 0 times it would reach the others
+            bool wild = false;
+            if (!full) {
+#pragma unroll
+                for (int i = 0; i < KB / 1024; ++i) {
+                    const u16x8 x = *reinterpret_cast<const u16x8 *>(Vs + i * 1024 + lane * 16);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) wild |= (x[e] & Mx<C>::kExp) == Mx<C>::kExp;
+                }
+                wild = __any(wild);
+            }
+            if (!wild) {
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    v8 ph, pl;
+                    l += weights(c, ph, pl);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const v8 v = v_at(c, d);
+                        o[d] = Mx<C>::mm(v, ph, o[d]);
+                        if constexpr (kSplit) o[d] = Mx<C>::mm(v, pl, o[d]);
+                    }
+                }
+            } else {  // finite values as above; rows that see one that is not become NaN there
+#pragma unroll 1
+                for (int d = 0; d < ND; ++d) {
+                    acc hit, od;
+#pragma unroll
+                    for (int i = 0; i < AV; ++i) hit[i] = od[i] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < NC; ++c) {
+                        u16x8 v = __builtin_bit_cast(u16x8, v_at(c, d)), w, seen;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool out = (v[e] & Mx<C>::kExp) == Mx<C>::kExp;
+                            w[e] = out ? Mx<C>::kOne : 0;
+                            v[e] = out ? 0 : v[e];
+                            const int key = kt + (NQ == 32 ? key_in(c / 2, (8 * c + e) & 15) : key_in(2 * c + e / 4, e & 3));
+                            seen[e] = uint32_t(key - see.begin) < see_n ? Mx<C>::kOne : 0;
+                        }
+                        v8 ph, pl;
+                        const float sum = weights(c, ph, pl);
+                        l += d == 0 ? sum : 0.f;
+                        od = Mx<C>::mm(__builtin_bit_cast(v8, v), ph, od);
+                        if constexpr (kSplit) od = Mx<C>::mm(__builtin_bit_cast(v8, v), pl, od);
+                        hit = Mx<C>::mm(__builtin_bit_cast(v8, w), __builtin_bit_cast(v8, seen), hit);
+                    }
+#pragma unroll
+                    for (int x = 0; x < ND; ++x)
+#pragma unroll
+                        for (int i = 0; i < AV; ++i)
+                            if (x == d) o[x][i] += hit[i] > 0.f ? __builtin_nanf("") : od[i];
+                }
+            }
+        }
+        if constexpr (WQ > 1) read_barrier();
+    }
+    raise_status(a.status, bad_page, kStatusBadPage);
+    l = rows_sum<NQ>(l);
+
+    T *out = static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * hd;
+    const int64_t part = (int64_t(row) * a.heads + head) * a.slots + slot0 + split;
+    if constexpr (WK == 1) {
+        if (!valid) return;
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        if (!whole && lh == 0) {
+            a.ml[2 * part] = m;
+            a.ml[2 * part + 1] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < AV; i += 4) {
+                const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
+                if (e >= hd) continue;
+                const f32x4 x = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+                if (whole) store4(out + e, x * inv);
+                else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
+            }
+    } else {
+        // the waves' parts: maxima and sums, then every wave's rows scaled to the common maximum, added in wave order
+        constexpr int LDO = HDP + 4;
+        float *sm = reinterpret_cast<float *>(smem), *so = sm + 2 * WK * NQ;
+        wait_step<0>();
+        block_barrier();  // every stream has been read
+        if (lh == 0) {
+            sm[wk * NQ + col] = m;
+            sm[(WK + wk) * NQ + col] = l;
+        }
+        wait_step<0>();
+        block_barrier();
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * NQ + col]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) L += sm[w * NQ + col] == -INFINITY ? 0.f : exp2_fast(sm[w * NQ + col] - M) * sm[(WK + w) * NQ + col];
+        const float f = m == -INFINITY ? 0.f : exp2_fast(m - M);
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int i = 0; i < AV; i += 4) {
+                const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
+                *reinterpret_cast<f32x4 *>(so + (wk * NQ + col) * LDO + e) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]} * f;
+            }
+        wait_step<0>();
+        block_barrier();
+        if (!valid) return;
+        const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+        if (!whole && wave == 0 && lh == 0) {
+            a.ml[2 * part] = M;
+            a.ml[2 * part + 1] = L;
+        }
+        // lane (col, lh) of wave w takes 4 dims at 4 (w (64 / NQ) + lh), and every 4 x 256 / NQ on
+        for (int e = 4 * (wave * (64 / NQ) + lh); e < hd; e += 4 * 256 / NQ) {
+            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WK; ++w) x += *reinterpret_cast<const f32x4 *>(so + (w * NQ + col) * LDO + e);
+            if (whole) store4(out + e, x * inv);
+            else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
+        }
+    }
+}
+
+// The parts of rows whose keys went in several runs, or partly with a group: M = their largest maximum, sums and outputs scaled
+// by 2^(max - M) and added in slot order. grid x = rows x ceil(heads / 8), block 256: 32 lanes a head, 4 dims each.
+template <class T>
+__global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
+    const int hb = (a.heads + 7) / 8, row = int(blockIdx.x) / hb, head = int(blockIdx.x) % hb * 8 + int(threadIdx.x) / 32;
+    const int e = 4 * (int(threadIdx.x) % 32);
     const int32_t s = find_seq(a.b, row);
     if (s < 0) return;
-    const SeqRows sr = seq_rows(a.b, a.c.shift, s);
-    raise_status(a.status, !sr.ok, kStatusBadBatch);
-    const int32_t pos = sr.len - sr.n + (row - sr.first);
-    const Span sp = visible(pos, sr.len, a.prefix ? a.prefix[s] : 0, a.window);
+    const Segment seg = seq_segment(a.b, a.p, a.c.shift, s);
     const int32_t grp = group_of(a.p, s);
-    const int32_t shared = grp >= 0 ? a.p.len[grp] : 0;
-    const int32_t *tab = a.b.table + int64_t(s) * a.b.page_ld;
-    const int32_t *ptab = grp >= 0 ? a.b.table + int64_t(clamp_i32(a.p.seq_start[grp], 0, a.b.seqs - 1)) * a.b.page_ld : tab;
-    const bool on0 = lane < hd, on1 = lane + 64 < hd;
-    const T *q = static_cast<const T *>(a.q) + int64_t(row) * a.ld_q + int64_t(h) * hd;
-    const float q0 = on0 ? float(q[lane]) : 0.f, q1 = on1 ? float(q[lane + 64]) : 0.f;
-    const float slope = a.slopes ? a.slopes[h] : 0.f;
-    float mx = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int32_t j = sp.begin + w; j < sp.end; j += 4) {
-        const int32_t page = page_of(a.c, j < shared ? ptab : tab, j);
-        if (page < 0) {
-            raise_status(a.status, lane == 0, kStatusBadPage);
-            continue;
-        }
-        const int64_t off = key_offset(a.c, page, g, j);
-        const C *kr = static_cast<const C *>(a.c.k) + off, *vr = static_cast<const C *>(a.c.v) + off;
-        float sc = a.scale * wave_sum((on0 ? q0 * float(kr[lane]) : 0.f) + (on1 ? q1 * float(kr[lane + 64]) : 0.f));
-        if (a.cap > 0.f) sc = a.cap * tanhf(sc / a.cap);
-        sc -= slope * fabsf(float(pos - j));
-        const float mn = fmaxf(mx, sc), corr = expf(mx - mn), p = expf(sc - mn);
-        o0 = o0 * corr + (on0 ? p * float(vr[lane]) : 0.f);
-        o1 = o1 * corr + (on1 ? p * float(vr[lane + 64]) : 0.f);
-        l = l * corr + p;
-        mx = mn;
+    const int32_t gn = grp >= 0 ? runs_of(0, clamp_i32(a.p.len[grp], 0, a.b.page_ld << a.c.shift), a.gsplits, a.gleast).count : 0;
+    const int32_t sn = runs_of(seg.key0, seg.key1, a.ssplits, a.sleast).count;
+    if (gn == 0 && sn <= 1) return;  // written by its only run
+    if (head >= a.heads || e >= a.c.hd) return;
+    const int64_t base = (int64_t(row) * a.heads + head) * a.slots;
+    auto slot = [&](int i) { return base + (i < gn ? i : a.gsplits + i - gn); };
+    float M = -INFINITY;
+    for (int i = 0; i < gn + sn; ++i) M = fmaxf(M, a.ml[2 * slot(i)]);
+    float L = 0.f;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < gn + sn; ++i) {
+        const int64_t at = slot(i);
+        const float mi = a.ml[2 * at], li = a.ml[2 * at + 1];
+        const f32x4 oi = *reinterpret_cast<const f32x4 *>(a.po + at * a.c.hd + e);
+        const float f = mi == -INFINITY ? 0.f : exp2_fast(mi - M);
+        L += f * li;
+        x += oi * f;
     }
-    __shared__ float sm_m[4], sm_l[4], sm_o[4][128];
-    if (lane == 0) {
-        sm_m[w] = mx;
-        sm_l[w] = l;
-    }
-    sm_o[w][lane] = o0;
-    sm_o[w][lane + 64] = o1;
-    __syncthreads();
-    if (int(threadIdx.x) >= hd) return;
-    float M = -INFINITY, L = 0.f, O = 0.f;
-    for (int i = 0; i < 4; ++i) M = fmaxf(M, sm_m[i]);
-    for (int i = 0; i < 4; ++i) {
-        if (sm_m[i] == -INFINITY) continue;
-        const float f = expf(sm_m[i] - M);
-        L += f * sm_l[i];
-        O += f * sm_o[i][threadIdx.x];
-    }
-    static_cast<T *>(a.out)[int64_t(row) * a.ld_out + int64_t(h) * hd + threadIdx.x] = T(L > 0.f || L != L ? O / L : 0.f);
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    store4(static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * a.c.hd + e, x * inv);
 }
 
 }  // namespace vh

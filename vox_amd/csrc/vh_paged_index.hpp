@@ -76,4 +76,59 @@ VH_HD int32_t group_of(const PagedGroups &p, int32_t s) {
     return -1;
 }
 
+// ------------------------------------------------------------------ the attention's work
+// A segment is what meets one run of keys: the rows of a group and its shared keys, or the rows of a sequence and its own
+// keys behind the shared ones. Its query rows are (row, head of the kv head's `group` heads), the head fastest; a tile is
+// `tile` of them. The keys go in runs (split_of), one per split; a (query row, segment) pair leaves one part per run.
+struct Segment {
+    int32_t row0, rows;  // rows of the batch
+    int32_t seq0, seq1;  // their sequences
+    int32_t key0, key1;  // keys, from the page table of seq0
+    bool ok;
+};
+VH_HD Segment group_segment(const PagedBatch &b, const PagedGroups &p, int32_t shift, int32_t g) {
+    Segment s;
+    s.seq0 = clamp_i32(p.seq_start[g], 0, b.seqs);
+    s.seq1 = clamp_i32(p.seq_start[g + 1], s.seq0, b.seqs);
+    s.row0 = clamp_i32(b.row_start[s.seq0], 0, b.rows);
+    s.rows = clamp_i32(b.row_start[s.seq1], s.row0, b.rows) - s.row0;
+    s.key0 = 0;
+    s.key1 = clamp_i32(p.len[g], 0, b.page_ld << shift);
+    s.ok = s.seq0 == p.seq_start[g] && s.seq1 == p.seq_start[g + 1] && s.key1 == p.len[g];
+    return s;
+}
+VH_HD Segment seq_segment(const PagedBatch &b, const PagedGroups &p, int32_t shift, int32_t seq) {
+    const SeqRows r = seq_rows(b, shift, seq);
+    const int32_t g = group_of(p, seq), shared = g >= 0 ? p.len[g] : 0;
+    Segment s;
+    s.seq0 = seq;
+    s.seq1 = seq + 1;
+    s.row0 = r.first;
+    s.rows = r.n;
+    s.key0 = clamp_i32(shared, 0, r.len);
+    s.key1 = r.len;
+    s.ok = r.ok;
+    return s;
+}
+// Keys [key0, key1) in at most `splits` runs of a multiple of kKeyTile keys, of at least `least` (a multiple too), whose borders
+// but the first and last are multiples of kKeyTile.
+constexpr int32_t kKeyTile = 64;
+struct Runs {
+    int32_t first, step, count;  // run i: keys [max(key0, first + i step), min(key1, first + (i + 1) step))
+};
+VH_HD Runs runs_of(int32_t key0, int32_t key1, int32_t splits, int32_t least) {
+    Runs r;
+    r.first = key0 & ~(kKeyTile - 1);
+    const int64_t keys = int64_t(key1) - r.first;
+    const int64_t even = ((keys + splits - 1) / splits + kKeyTile - 1) & ~int64_t(kKeyTile - 1);
+    r.step = int32_t(even > least ? even : least);
+    r.count = key1 > key0 ? int32_t((keys + r.step - 1) / r.step) : 0;
+    return r;
+}
+VH_HD Span run_at(const Runs &r, int32_t key0, int32_t key1, int32_t i) {
+    const int64_t a = r.first + int64_t(i) * r.step, e = a + r.step;
+    return Span{a > key0 ? int32_t(a) : key0, e < key1 ? int32_t(e) : key1};
+}
+VH_HD int32_t tiles_of(int32_t rows, int32_t group, int32_t tile) { return int32_t((int64_t(rows) * group + tile - 1) / tile); }
+
 }  // namespace vh

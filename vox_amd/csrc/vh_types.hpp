@@ -9,7 +9,7 @@ namespace vh {
 // The library's range-status word: a kernel whose arithmetic cannot represent a value it was given sets a bit, and
 // the synchronous entry points fail the call when one is set (so the engine computes it on the CPU instead).
 // kStatusBadPage / kStatusBadBatch: a page table, or a ragged batch's row_start / len, that names what is not there (the
-// kernel leaves those keys out and touches nothing outside its buffers).
+// kernel touches nothing outside its buffers).
 enum : int32_t { kStatusF16Range = 1, kStatusFixRange = 2, kStatusBadPage = 4, kStatusBadBatch = 8 };
 
 // GEMV input prologues: x as is; RMSNorm(x, gamma); or the merge of split-K attention partials.
@@ -338,6 +338,18 @@ struct PagedAttnArgs {
     int32_t heads, window;
     float scale, cap;
     int32_t *status;
+    // the parts of rows whose keys go in several runs: slots of a (row, head), a group's gsplits then a sequence's ssplits; ml
+    // (max, sum) and po [head_dim] of each, behind each other in one workspace
+    float *ml, *po;
+    int32_t slots, gsplits, ssplits, gleast, sleast;
+};
+// Where the attention's launches come from: tiles and splits by the batch's bounds, and the floats of its workspace.
+struct PagedPlan {
+    int32_t stile, gtile;    // query rows of a tile of a sequence, of a group (0: no groups)
+    int32_t stiles, gtiles;  // at most so many tiles
+    bool direct;             // tile i is sequence i
+    int32_t gsplits, ssplits, gleast, sleast, slots;
+    int64_t ws_floats;
 };
 
 }  // namespace vh

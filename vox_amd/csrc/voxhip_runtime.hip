@@ -215,6 +215,9 @@ struct Ctx {
     // the range-status word (allocated and zeroed at init) and its pinned host copy; word 1 of the device block is
     // the scratch of the weight max |w| reduction
     int32_t *status_dev = nullptr, *status_pin = nullptr;
+    // parts of the paged-cache attention (paged_ws)
+    float *paged_ws = nullptr;
+    int64_t paged_ws_floats = 0;
     // VOXHIP_CHECK_HOST=1 at a voxhip_init call: copy_h2d / copy_d2h check each side's memory type (check_copy_side)
     bool check_copies = false;
 };
@@ -3981,6 +3984,19 @@ void need_rows(const void *p, int64_t ld, int64_t cols, int32_t type, const char
     if (ld % 8) paged_fail(std::string(what) + ": the row stride is not a multiple of 8");
 }
 
+// The attention's parts, grown when a batch needs more (work in flight on the stream uses the old block until it is waited for).
+float *paged_ws(int64_t floats) {
+    if (g.paged_ws_floats < floats) {
+        HIPCHECK(hipStreamSynchronize(g.stream));
+        dfree(g.paged_ws);
+        g.paged_ws = nullptr;
+        g.paged_ws_floats = 0;
+        g.paged_ws = dalloc_t<float>(size_t(floats));
+        g.paged_ws_floats = floats;
+    }
+    return g.paged_ws;
+}
+
 int kv_append(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r) {
     AppendArgs a{};
     a.c = paged_kv(kv);
@@ -4052,7 +4068,8 @@ int attn_paged(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const vox
     require_ok();
     const OnDevice on;
     vh::prof_stage("paged");
-    HIPCHECK(launch_paged_attn(r->type, a, g.stream));
+    const PagedPlan plan = plan_paged_attn(a, b->max_rows, b->max_len, p ? p->max_len : 0);
+    HIPCHECK(launch_paged_attn(r->type, a, plan, paged_ws(plan.ws_floats), g.stream));
     return 1;
 }
 }  // namespace
