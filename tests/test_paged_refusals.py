@@ -38,7 +38,7 @@ BOTH = [
     (dict(kv_head_dim=136), "head_dim"), (dict(kv_head_dim=60), "head_dim"), (dict(kv_head_dim=0), "head_dim"),
     (dict(kv_page_size=24), "page_size"), (dict(kv_page_size=4), "page_size"), (dict(kv_page_size=2048), "page_size"),
     (dict(kv_pages=0), "no pages"), (dict(kv_kv_heads=0), "kv_heads"), (dict(kv_kv_heads=3), "overlap"),
-    (dict(kv_pos_stride=56), "strides"), (dict(kv_pos_stride=68), "strides"), (dict(kv_page_stride=-2048), "strides"),
+    (dict(kv_pos_stride=56), "strides"), (dict(kv_pos_stride=68), "strides"), (dict(kv_page_stride=-2048), "strides"), (dict(kv_pos_stride=(1 << 26) + 8), "too large"),
     (dict(kv_head_stride=64), "overlap"), (dict(kv_page_stride=1024), "pages overlap"), (dict(kv_page_stride=1 << 60), "too large"),
     (dict(kv_k=None), "k is missing"), (dict(kv_v=None), "v is missing"), (dict(kv_k=A + 8), "k is not aligned"),
     (dict(b_seqs=-1), "out of range"), (dict(b_rows=-1), "out of range"), (dict(b_rows=(1 << 24) + 1), "out of range"),

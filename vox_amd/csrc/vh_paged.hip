@@ -55,46 +55,56 @@ PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_
         p.gsplits = splits_for(std::max<int64_t>(1, q / p.gtile), std::max(max_shared, 1));
     }
     p.slots = p.gsplits + p.ssplits;
-    p.ws_floats = p.gsplits || p.ssplits > 1 ? int64_t(a.b.rows) * a.heads * p.slots * (2 + a.c.hd) : 0;
+    p.ws_floats = p.gsplits || p.ssplits > 1 ? int64_t(a.b.rows) * a.heads * p.slots * (2 + a.c.hd) + a.b.rows : 0;
     return p;
 }
 
 namespace {
-template <class T, class C, int HDP, int NQ, int WQ, bool GROUPS>
-hipError_t attn_launch(const PagedAttnArgs &a, int32_t tiles, int32_t splits, int32_t least, bool direct, hipStream_t s) {
-    constexpr size_t pitch = HDP <= 64 ? 128 : 256, stages = size_t(4 / WQ) * 2 * 2 * (WQ == 4 ? 64 : 32) * pitch;
-    constexpr size_t join = WQ == 4 ? 0 : (size_t(2) * 4 * NQ + size_t(4) * NQ * (HDP + 4)) * 4, smem = stages > join ? stages : join;
-    const int64_t grid = int64_t(tiles) * splits * a.c.kv_heads;
+template <class T, class C, int HDP, int GN, int GW, int SN, int SW>
+hipError_t attn_launch(const PagedAttnArgs &a, hipStream_t s) {
+    constexpr size_t pitch = HDP <= 64 ? 128 : 256, stages = size_t(256) * pitch;  // of either kind of tile
+    constexpr size_t nq = GN > SN ? GN : SN, join = (size_t(2) * 4 * nq + size_t(4) * nq * (HDP + 4)) * 4;
+    constexpr bool joins = GW == 1 || SW == 1;
+    constexpr size_t smem = joins && join > stages ? join : stages;
+    const int64_t grid = (int64_t(GN ? a.gtiles : 0) * a.gsplits + int64_t(a.stiles) * a.ssplits) * a.c.kv_heads;
     if (grid > INT32_MAX) return hipErrorInvalidValue;
-    auto *k = k_paged_attn<T, C, HDP, NQ, WQ, GROUPS>;
+    auto *k = k_paged_attn<T, C, HDP, GN, GW, SN, SW>;
     if (const hipError_t e = ensure_smem(reinterpret_cast<const void *>(k), smem); e != hipSuccess) return e;
-    return launch(k, dim3(unsigned(grid)), dim3(256), smem, s, a, tiles, splits, least, int32_t(direct));
+    return launch(k, dim3(unsigned(grid)), dim3(256), smem, s, a);
 }
 template <class T, class C, int HDP>
-hipError_t attn_of(const PagedAttnArgs &a, const PagedPlan &p, hipStream_t s) {
-    hipError_t e = hipSuccess;
-    if (p.gtile == 16) e = attn_launch<T, C, HDP, 16, 1, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
-    else if (p.gtile == 32) e = attn_launch<T, C, HDP, 32, 1, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
-    else if (p.gtile) e = attn_launch<T, C, HDP, 32, 4, true>(a, p.gtiles, p.gsplits, p.gleast, false, s);
-    if (e != hipSuccess) return e;
-    if (p.stile == 16) return attn_launch<T, C, HDP, 16, 1, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
-    if (p.stile == 32) return attn_launch<T, C, HDP, 32, 1, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
-    return attn_launch<T, C, HDP, 32, 4, false>(a, p.stiles, p.ssplits, p.sleast, p.direct, s);
+hipError_t attn_of(const PagedAttnArgs &a, int gtile, int stile, hipStream_t s) {
+    if (gtile == 0) {
+        if (stile == 16) return attn_launch<T, C, HDP, 0, 0, 16, 1>(a, s);
+        if (stile == 32) return attn_launch<T, C, HDP, 0, 0, 32, 1>(a, s);
+        return attn_launch<T, C, HDP, 0, 0, 32, 4>(a, s);
+    }
+    if (gtile == 16) return attn_launch<T, C, HDP, 16, 1, 16, 1>(a, s);
+    if (gtile == 32 && stile == 16) return attn_launch<T, C, HDP, 32, 1, 16, 1>(a, s);
+    if (gtile == 32) return attn_launch<T, C, HDP, 32, 1, 32, 1>(a, s);
+    if (stile == 16) return attn_launch<T, C, HDP, 32, 4, 16, 1>(a, s);
+    if (stile == 32) return attn_launch<T, C, HDP, 32, 4, 32, 1>(a, s);
+    return attn_launch<T, C, HDP, 32, 4, 32, 4>(a, s);
 }
 }  // namespace
 
 hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &p, float *ws, hipStream_t s) {
-    if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0 || (p.ws_floats && !ws)) return hipErrorInvalidValue;
+    if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0 || (p.ws_floats && !ws) || p.slots > 64) return hipErrorInvalidValue;
     const int64_t join = int64_t(a.b.rows) * ((a.heads + 7) / 8);
     if (join > INT32_MAX) return hipErrorInvalidValue;
     a.status = status_word();
     a.slots = p.slots; a.gsplits = p.gsplits; a.ssplits = p.ssplits; a.gleast = p.gleast; a.sleast = p.sleast;
-    a.po = ws;  // 16-byte aligned rows first
-    a.ml = ws ? ws + int64_t(a.b.rows) * a.heads * p.slots * a.c.hd : nullptr;
+    a.gtiles = p.gtiles; a.stiles = p.stiles; a.direct = p.direct;
+    if (p.ws_floats) {
+        const int64_t parts = int64_t(a.b.rows) * a.heads * p.slots;
+        a.po = ws;  // 16-byte aligned rows first
+        a.ml = ws + parts * a.c.hd;
+        a.desc = reinterpret_cast<int32_t *>(a.ml + 2 * parts);
+    }
     return by_type(type, [&](auto t, auto c) {
         using T = decltype(t);
         using C = decltype(c);
-        const hipError_t e = a.c.hd <= 64 ? attn_of<T, C, 64>(a, p, s) : a.c.hd <= 96 ? attn_of<T, C, 96>(a, p, s) : attn_of<T, C, 128>(a, p, s);
+        const hipError_t e = a.c.hd <= 64 ? attn_of<T, C, 64>(a, p.gtile, p.stile, s) : attn_of<T, C, 128>(a, p.gtile, p.stile, s);
         if (e != hipSuccess || !p.ws_floats) return e;
         return launch(k_paged_join<T>, dim3(unsigned(join)), dim3(256), 0, s, a);
     });

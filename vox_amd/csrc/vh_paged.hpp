@@ -136,9 +136,13 @@ struct Mx<__bf16> {
 // What lanes without a key (behind a sequence's last, past head_dim) read instead.
 static __device__ __align__(16) uint32_t kZero16[4];
 
-// 16 bytes per lane from its own address to LDS lds + 16 lane; as dma_b128, the waits are the caller's.
+// 16 bytes per lane to LDS lds + 16 lane, from its own address, or from a common one and its own 32-bit offset (s_nop: an
+// address that a vector instruction wrote into scalar registers needs 5 cycles); as dma_b128, the waits are the caller's.
 VH_DEV void dma_lane16(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(src) : "memory", "m0");
+}
+VH_DEV void dma_off16(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 // Every LDS read of this wave has returned, then the block's barrier.
 VH_DEV void read_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -166,17 +170,37 @@ VH_DEV float rows_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh to about 2^-23 of its value: odd polynomial (Taylor, to x^11) below 0.3, (1 - t) / (1 + t) with t = 2^(-2 |x| log2 e)
-// above, where 1 - t cancels little.
+// tanh as (1 - t) / (1 + t), t = 2^(-2 |x| log2 e): off by about 2^-24 absolutely. FINE: by about 2^-23 of its value also near
+// zero, where 1 - t cancels: an odd polynomial (Taylor, to x^11) below 0.3. Both are computed and one is taken: no branch.
+template <bool FINE>
 VH_DEV float tanh_f(float x) {
-    const float a = fabsf(x), x2 = x * x;
-    const float t = exp2_fast(-2.8853900817779268f * a);
-    const float big = copysignf((1.f - t) / (1.f + t), x);
+    const float a = fabsf(x), t = exp2_fast(-2.8853900817779268f * a);
+    float big = copysignf((1.f - t) * __builtin_amdgcn_rcpf(1.f + t), x);
+    if constexpr (!FINE) return big;
+    const float x2 = x * x;
     float p = fmaf(x2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
     p = fmaf(x2, p, -17.0f / 315.0f);
     p = fmaf(x2, p, 2.0f / 15.0f);
     p = fmaf(x2, p, -1.0f / 3.0f);
-    return a < 0.3f ? fmaf(x * x2, p, x) : big;
+    p = fmaf(x * x2, p, x);
+    asm volatile("" : "+v"(big), "+v"(p));
+    return a < 0.3f ? p : big;
+}
+
+// The group of sequence s (the first that holds it) and its shared keys, or -1 and 0: 64 groups at a time.
+VH_DEV int32_t find_group(const PagedGroups &p, int32_t s, int64_t most, int32_t *shared) {
+    const int lane = threadIdx.x & 63;
+    for (int32_t base = 0; base < p.groups; base += 64) {
+        const int32_t g = min(base + lane, p.groups - 1), n = p.len[g];
+        const uint64_t in = __ballot(base + lane < p.groups && s >= p.seq_start[g] && s < p.seq_start[g + 1]);
+        if (in) {
+            const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
+            *shared = clamp_i32(__builtin_amdgcn_readlane(n, l), 0, most);
+            return base + l;
+        }
+    }
+    *shared = 0;
+    return -1;
 }
 
 // The segment (of n, with rows_of(i) rows each) and the tile in it of the launch's tile t: 64 segments at a time.
@@ -220,13 +244,13 @@ VH_DEV bool find_tile(int32_t n, int32_t t, int32_t group, int32_t tile, F rows_
 // 2^(s - m + kUp) with m within 2^kLag of the running maximum: the running maximum only moves (and O^T is only rescaled) when a
 // score passes it by more than kLag, and kUp keeps small f16 weights out of the subnormals.
 template <class T, class C, int HDP, int NQ, int WQ, bool GROUPS>
-__global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnArgs a, int32_t tiles, int32_t splits, int32_t least, int32_t direct) {
+VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     typedef typename Mx<C>::v8 v8;
     typedef typename std::conditional<NQ == 32, f32x16, f32x4>::type acc;
     constexpr bool kSplit = std::is_same<T, float>::value;
     constexpr int WK = 4 / WQ, KW = WQ == 4 ? 64 : 32, TILE = NQ * WQ;
     constexpr int PITCH = HDP <= 64 ? 128 : 256, CPR = PITCH / 16, R = 64 / CPR;  // bytes of a key in LDS, its pieces, keys a DMA
-    constexpr int KB = KW * PITCH, STAGE = 2 * KB;                                // K then V of a tile
+    constexpr int KB = KW * PITCH, STAGE = 2 * KB, STAGES = WQ == 4 ? 2 : 1;      // K then V of a tile
     constexpr int NI = KW / R / WQ;                                               // DMAs of K (and of V) a wave and tile
     constexpr int KD = NQ == 32 ? 16 : 32;                                        // K of one product
     constexpr int SUB = NQ, NSUB = KW / SUB, AV = NQ == 32 ? 16 : 4;              // keys of one S^T product, values a lane
@@ -234,45 +258,48 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
     constexpr int NC = KW / KD;                                                   // P^T operands
     constexpr float kUp = std::is_same<C, __bf16>::value ? 0.f : 6.f, kLag = 8.f;
     static_assert(NI >= 1 && (NI % 2 == 0 || R == 8), "the swizzle's parity is the DMA's");
-    extern __shared__ __align__(16) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     const int wq = wave % WQ, wk = wave / WQ, col = lane % NQ, lh = lane / NQ;  // lh: which rows of a product this lane holds
     const int G = a.c.kv_heads, group = a.heads / G, hd = a.c.hd;
     const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>((lds_void *)smem));
+    const int32_t splits = GROUPS ? a.gsplits : a.ssplits;
     // kv heads are the fastest index: blocks of one kv head (and its keys) meet in few XCDs' L2
-    int id = blockIdx.x;
     const int g = id % G;
     id /= G;
     const int split = id % splits;
-    int32_t t = id / splits, seg_id = t, local = 0;
+    int32_t t = id / splits, seg_id = t, local = 0, shared = 0;
     Segment seg;
+    bool whole = false;  // a row whose keys are one run is written here, otherwise its parts are joined by k_paged_join
+    Runs runs;
     if constexpr (GROUPS) {
         if (!find_tile(a.p.groups, t, group, TILE, [&](int32_t i) { return group_segment(a.b, a.p, a.c.shift, i).rows; }, &seg_id, &local)) return;
         seg = group_segment(a.b, a.p, a.c.shift, seg_id);
+        runs = runs_of(seg.key0, seg.key1, splits, a.gleast);
     } else {
-        t = tiles - 1 - t;  // the last tiles of a prompt see the most keys: first
+        t = a.stiles - 1 - t;  // the last tiles of a prompt see the most keys: first
         seg_id = t;
-        if (!direct && !find_tile(a.b.seqs, t, group, TILE,
-                                  [&](int32_t i) {
-                                      const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
-                                      return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
-                                  },
-                                  &seg_id, &local))
+        if (!a.direct && !find_tile(a.b.seqs, t, group, TILE,
+                                    [&](int32_t i) {
+                                        const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
+                                        return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
+                                    },
+                                    &seg_id, &local))
             return;
-        seg = seq_segment(a.b, a.p, a.c.shift, seg_id);
+        const SeqRows sr = seq_rows(a.b, a.c.shift, seg_id);
+        find_group(a.p, seg_id, a.b.page_ld << a.c.shift, &shared);
+        seg = Segment{sr.first, sr.n, seg_id, seg_id + 1, min(shared, sr.len), sr.len, sr.ok};
+        runs = runs_of(seg.key0, seg.key1, splits, a.sleast);
     }
     const int32_t qrows = seg.rows * group;
-    raise_status(a.status, threadIdx.x == 0 && (!seg.ok || (direct && qrows > TILE)), kStatusBadBatch);
+    raise_status(a.status, threadIdx.x == 0 && (!seg.ok || (!GROUPS && a.direct && qrows > TILE)), kStatusBadBatch);
     if (local * TILE >= qrows) return;
-    const Runs runs = runs_of(seg.key0, seg.key1, splits, least);
-    // a row whose keys are one run is written here, otherwise its parts are joined by k_paged_join
-    bool whole = false;
-    int32_t slot0 = 0;
     if constexpr (!GROUPS) {
-        const int32_t grp = group_of(a.p, seg_id);
-        const Runs gr = grp >= 0 ? runs_of(0, clamp_i32(a.p.len[grp], 0, a.b.page_ld << a.c.shift), a.gsplits, a.gleast) : Runs{0, 0, 0};
-        whole = gr.count == 0 && runs.count <= 1;
-        slot0 = a.gsplits;
+        const int32_t gruns = runs_of(0, shared, a.gsplits, a.gleast).count;
+        whole = gruns == 0 && runs.count <= 1;
+        if (a.desc && split == 0 && g == 0) {  // what the join will find
+            const int32_t first = local * TILE / group, i = first + int(threadIdx.x);
+            if (i * group < min(local * TILE + TILE, qrows) && i < seg.rows) a.desc[seg.row0 + i] = whole ? 0 : gruns | runs.count << 16;
+        }
     }
     if (split >= runs.count && !(whole && split == 0)) return;
     const Span run = runs.count ? run_at(runs, seg.key0, seg.key1, split) : Span{0, 0};
@@ -281,9 +308,26 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
     const int32_t u = local * TILE + wq * NQ + col;
     const bool valid = u < qrows;
     const int32_t tok = valid ? u / group : 0, row = seg.row0 + tok, head = g * group + (valid ? u - tok * group : 0);
-    int32_t seq = seg.seq0;
-    if constexpr (GROUPS) {  // the sequence that holds the row: by the guess of one row each, or halving
-        seq = min(seg.seq0 + tok, seg.seq1 - 1);
+    // the queries, raw: needed only after the first keys are on their way
+    constexpr int NK = HDP / KD;
+    u32x4 qraw[NK][kSplit ? 2 : 1];
+    {
+        const T *qr = static_cast<const T *>(a.q) + int64_t(row) * a.ld_q + int64_t(head) * hd;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            const int d = KD * c + 8 * lh;
+            const bool in = valid && d < hd;
+            qraw[c][0] = in ? *reinterpret_cast<const u32x4 *>(qr + d) : u32x4{0u, 0u, 0u, 0u};
+            if constexpr (kSplit) qraw[c][1] = in ? *reinterpret_cast<const u32x4 *>(qr + d + 4) : u32x4{0u, 0u, 0u, 0u};
+        }
+    }
+    const float slope_raw = a.slopes ? a.slopes[head] : 0.f;
+    int32_t pos, lo_any, hi_any, lo_all, hi_all;  // of the wave's rows: the keys that any sees, and those that all see
+    int32_t kb = run.begin, ke = run.end;         // the block's keys
+    Span see;
+    if constexpr (GROUPS) {
+        // the sequence that holds the row: by the guess of one row each, or halving
+        int32_t seq = min(seg.seq0 + tok, seg.seq1 - 1);
         if (!(a.b.row_start[seq] <= row && row < a.b.row_start[seq + 1])) {
             int32_t lo = seg.seq0, hi = seg.seq1;  // the last s with row_start[s] <= row
             while (hi - lo > 1) {
@@ -293,115 +337,123 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
             }
             seq = lo;
         }
+        const SeqRows sr = seq_rows(a.b, a.c.shift, seq);
+        pos = sr.len - sr.n + (row - sr.first);
+        see = visible(pos, sr.len, a.prefix ? a.prefix[seq] : 0, a.window);
+        lo_any = run.begin;
+        hi_any = run.end;
+        const bool all = __all(!valid || (see.begin <= run.begin && see.end >= run.end));
+        lo_all = all ? run.begin : INT32_MAX;
+        hi_all = run.end;
+    } else {
+        // a sequence's rows see no less at either end the later they stand
+        const int32_t pf = a.prefix ? a.prefix[seg_id] : 0, len = seg.key1, before = len - seg.rows;
+        pos = before + tok;
+        see = visible(pos, len, pf, a.window);
+        auto at = [&](int32_t q) { return visible(before + min(q, qrows - 1) / group, len, pf, a.window); };
+        const int32_t w0 = local * TILE + wq * NQ;
+        const Span b0 = at(local * TILE), b1 = at(local * TILE + TILE - 1), first = at(w0), last = at(w0 + NQ - 1);
+        kb = max(kb, b0.begin);
+        ke = min(ke, b1.end);
+        lo_any = w0 < qrows ? max(first.begin, run.begin) : INT32_MAX;
+        hi_any = min(last.end, run.end);
+        lo_all = max(last.begin, run.begin);
+        hi_all = min(first.end, run.end);
     }
-    const SeqRows sr = seq_rows(a.b, a.c.shift, seq);
-    const int32_t pos = sr.len - sr.n + (row - sr.first);
-    Span see = visible(pos, sr.len, a.prefix ? a.prefix[seq] : 0, a.window);
     see.begin = max(see.begin, run.begin);
     see.end = valid ? min(see.end, run.end) : 0;
     if (see.begin >= see.end) see = Span{0, 0};
     const uint32_t see_n = uint32_t(see.end - see.begin);
-    // of the wave's rows: the keys that any sees, and those that all see
-    int32_t lo_any = see_n ? see.begin : INT32_MAX, hi_any = see.end, lo_all = valid ? (see_n ? see.begin : INT32_MAX) : 0,
-            hi_all = valid ? see.end : INT32_MAX;
-#pragma unroll
-    for (int o = 1; o < NQ; o <<= 1) {
-        lo_any = min(lo_any, __shfl_xor(lo_any, o, 64));
-        hi_any = max(hi_any, __shfl_xor(hi_any, o, 64));
-        lo_all = max(lo_all, __shfl_xor(lo_all, o, 64));
-        hi_all = min(hi_all, __shfl_xor(hi_all, o, 64));
-    }
-    lo_any = __builtin_amdgcn_readfirstlane(lo_any);
-    hi_any = __builtin_amdgcn_readfirstlane(hi_any);
-    lo_all = __builtin_amdgcn_readfirstlane(lo_all);
-    hi_all = __builtin_amdgcn_readfirstlane(hi_all);
-    // the block's keys: of a sequence's tile from its first and last row, of a group's the run
-    int32_t kb = run.begin, ke = run.end;
-    if constexpr (!GROUPS) {
-        const int32_t t0 = local * TILE / group, t1 = min(local * TILE + TILE, qrows) - 1, pf = a.prefix ? a.prefix[seg_id] : 0;
-        const int32_t p0 = sr.len - sr.n + t0, p1 = sr.len - sr.n + t1 / group;
-        kb = max(kb, visible(p0, sr.len, pf, a.window).begin);
-        ke = min(ke, visible(p1, sr.len, pf, a.window).end);
-    }
     kb = __builtin_amdgcn_readfirstlane(kb & ~(KW * WK - 1));
     ke = __builtin_amdgcn_readfirstlane(ke);
 
-    // queries as the second operand of S^T: column col, K elements 8 lh .. of every product. A negative scale turns them
-    // around, so that the largest product is the largest score.
-    constexpr int NK = HDP / KD;
-    v8 qh[NK], ql[kSplit ? NK : 1];
-    {
-        const T *qr = static_cast<const T *>(a.q) + int64_t(row) * a.ld_q + int64_t(head) * hd;
-        const float sign = a.scale < 0.f ? -1.f : 1.f;
-        bool bad = false;
-#pragma unroll
-        for (int c = 0; c < NK; ++c) {
-            const int d = KD * c + 8 * lh;
-            const bool in = valid && d < hd;
-            if constexpr (kSplit) {
-                f32x4 x0 = {0.f, 0.f, 0.f, 0.f}, x1 = x0;
-                if (in) {
-                    x0 = *reinterpret_cast<const f32x4 *>(qr + d);
-                    x1 = *reinterpret_cast<const f32x4 *>(qr + d + 4);
-                }
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    _Float16 hi, lo;
-                    bad |= split_f16(sign * (e < 4 ? x0[e] : x1[e - 4]), hi, lo);
-                    qh[c][e] = hi;
-                    ql[c][e] = lo;
-                }
-            } else {
-                u32x4 x = {0u, 0u, 0u, 0u};
-                if (in) x = *reinterpret_cast<const u32x4 *>(qr + d);
-                const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-                qh[c] = __builtin_bit_cast(v8, x ^ u32x4{flip, flip, flip, flip});
-            }
-        }
-        raise_status(a.status, bad, kStatusF16Range);
-    }
     constexpr float kLog2e = 1.44269504088896341f;
     const bool capped = a.cap > 0.f, biased = a.slopes != nullptr;
     const float sc = fabsf(a.scale) * (capped ? 1.f / a.cap : kLog2e), cap2 = a.cap * kLog2e;
-    const float slope = biased ? a.slopes[head] * kLog2e : 0.f;
+    const float slope = slope_raw * kLog2e;
 
     // DMA: this lane's key of R and piece of CPR, by the DMA's parity where the swizzle needs it
     const int rin = lane / CPR, piece = lane % CPR;
-    int64_t voff[2];
+    uint32_t voff[2];
     bool vin[2];
 #pragma unroll
     for (int par = 0; par < 2; ++par) {
         const int p = PITCH == 256 ? piece ^ (((4 * par + rin) & 7) << 1) : piece ^ (((rin >> 1) & 3) << 1);
-        voff[par] = (int64_t(rin) * a.c.pos_stride + 8 * p) * 2;
+        voff[par] = (uint32_t(rin) * uint32_t(a.c.pos_stride) + 8 * p) * 2;
         vin[par] = 8 * p < hd;
     }
     const int32_t *tab = a.b.table + int64_t(seg.seq0) * a.b.page_ld;
     const int32_t last_page = run.end > run.begin ? (run.end - 1) >> a.c.shift : 0, first_page = run.begin >> a.c.shift;
     int32_t pg = -1, pbase = -64;  // lane l: the page of table entry pbase + l
     bool bad_page = false;
-    auto issue = [&](int32_t kt, uint32_t buf) {
-        const int32_t i0 = max(kt >> a.c.shift, first_page), i1 = min((kt + KW - 1) >> a.c.shift, last_page);
+    // K (or V, by its pool's first byte of this kv head) of the keys kt .. kt + KW - 1 to buf. A tile inside the run, of whole
+    // pitches and pages of the pool, takes its addresses from scalars alone; otherwise lanes without a key read zeros.
+    const uint8_t *const kpool = static_cast<const uint8_t *>(a.c.k) + int64_t(g) * a.c.head_stride * 2;
+    const uint8_t *const vpool = static_cast<const uint8_t *>(a.c.v) + int64_t(g) * a.c.head_stride * 2;
+    const int64_t page_bytes = a.c.page_stride * 2;
+    const uint32_t pos_bytes = uint32_t(a.c.pos_stride) * 2;
+    const int shift = a.c.shift;
+    auto issue = [&](int32_t kt, const uint8_t *from, uint32_t buf) {
+        const int32_t i0 = max(kt >> shift, first_page), i1 = min((kt + KW - 1) >> shift, last_page);
         if (i0 < pbase || i1 >= pbase + 64) {
             pbase = i0;
             const int32_t i = i0 + lane;
             const bool in = i <= last_page;
             const int32_t e = in ? tab[i] : -1;
             pg = uint32_t(e) < uint32_t(a.c.pages) ? e : -1;
-            bad_page |= in && pg < 0;
+            bad_page |= __any(in && pg < 0);
         }
+        auto at = [&](int32_t page, int32_t key) { return int64_t(page) * page_bytes + int64_t(uint64_t(key & ((1 << shift) - 1)) * pos_bytes); };
+        if (hd == PITCH / 2 && !bad_page && kt >= run.begin && kt + KW <= run.end) {
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = wq * NI + n, par = n & 1;
-            const int32_t key = kt + R * i, pi = min(max(key >> a.c.shift, i0), i1);
-            const int32_t page = __builtin_amdgcn_readlane(pg, (pi - pbase) & 63);
-            const int64_t at = (int64_t(page) * a.c.page_stride + int64_t(g) * a.c.head_stride +
-                                int64_t(key & ((1 << a.c.shift) - 1)) * a.c.pos_stride) * 2 + voff[par];
-            const bool in = page >= 0 && vin[par] && key + rin >= run.begin && key + rin < run.end;
-            const void *zero = kZero16;
-            dma_lane16(in ? static_cast<const uint8_t *>(a.c.k) + at : zero, buf + i * 1024);
-            dma_lane16(in ? static_cast<const uint8_t *>(a.c.v) + at : zero, buf + KB + i * 1024);
+            for (int n = 0; n < NI; ++n) {
+                const int i = wq * NI + n;
+                const int32_t key = kt + R * i;
+                dma_off16(from + at(__builtin_amdgcn_readlane(pg, (key >> shift) - pbase), key), voff[n & 1], buf + i * 1024);
+            }
+        } else {
+#pragma unroll 2
+            for (int n = 0; n < NI; ++n) {
+                const int i = wq * NI + n;
+                const int32_t key = kt + R * i, mine = key + rin;
+                const int32_t page = __builtin_amdgcn_readlane(pg, (min(max(key >> shift, i0), i1) - pbase) & 63);
+                const bool in = page >= 0 && vin[n & 1] && mine >= run.begin && mine < run.end;
+                const uint8_t *zero = reinterpret_cast<const uint8_t *>(kZero16);
+                dma_lane16(in ? from + at(page, key) + voff[n & 1] : zero, buf + i * 1024);
+            }
         }
     };
+    // WQ = 4: two stages of K and V, the next tile on its way during this one. WQ = 1: one buffer each, refilled as soon as the
+    // wave has read it: K's during the softmax and V's product, V's during the next K's.
+    const uint32_t stream = uint32_t(wk) * STAGES * STAGE, buf0 = lds0 + stream;
+    const int32_t k_first = kb + wk * KW;
+    if (k_first < ke) {
+        issue(k_first, kpool, buf0);
+        issue(k_first, vpool, buf0 + KB);
+    }
+
+    // queries as the second operand of S^T: column col, K elements 8 lh .. of every product. A negative scale turns them
+    // around, so that the largest product is the largest score.
+    v8 qh[NK], ql[kSplit ? NK : 1];
+    {
+        bool bad = false;
+        const uint32_t flip = a.scale < 0.f ? (kSplit ? 0x80000000u : 0x80008000u) : 0u;
+#pragma unroll
+        for (int c = 0; c < NK; ++c) {
+            if constexpr (kSplit) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 hi, lo;
+                    bad |= split_f16(__uint_as_float(qraw[c][e / 4][e & 3] ^ flip), hi, lo);
+                    qh[c][e] = hi;
+                    ql[c][e] = lo;
+                }
+            } else {
+                qh[c] = __builtin_bit_cast(v8, qraw[c][0] ^ u32x4{flip, flip, flip, flip});
+            }
+        }
+        raise_status(a.status, bad, kStatusF16Range);
+    }
 
     acc o[ND];
 #pragma unroll
@@ -414,25 +466,29 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
     const int ksw = PITCH == 256 ? (col & 7) << 1 : ((col >> 1) & 3) << 1;
     const int vi = lane & 15, vkey = (NQ == 32 ? 4 * lh : 4 * (lane >> 4)) + (vi >> 2), vd = (NQ == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((vi & 3) >> 1);
     const int vsw = PITCH == 256 ? (vkey & 7) << 1 : ((vkey >> 1) & 3) << 1;
-    const uint32_t stream = uint32_t(wk) * 2 * STAGE;
     // value i of S^T product j: its key in the tile
     auto key_in = [&](int j, int i) { return SUB * j + (NQ == 32 ? (i & 3) + 8 * (i >> 2) + 4 * lh : i + 4 * lh); };
 
-    const int32_t k_first = kb + wk * KW;
-    const bool some = ke > kb;
-    if (some && k_first < ke) issue(k_first, lds0 + stream);
     int stage = 0;
-    for (int32_t kt = k_first; kt < ke; kt += KW * WK, stage ^= 1) {
-        const bool more = kt + KW * WK < ke;
-        if constexpr (WQ == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the other stage's reads are done
-        if (more) issue(kt + KW * WK, lds0 + stream + (stage ^ 1) * STAGE);
-        if (more) wait_step<2 * NI>();
-        else wait_step<0>();
-        if constexpr (WQ > 1) block_barrier();
+    for (int32_t kt = k_first; kt < ke; kt += KW * WK, stage ^= STAGES - 1) {
+        const int32_t next = kt + KW * WK;
+        const bool more = next < ke, seen = lo_any < kt + KW && hi_any > kt;
         const uint8_t *Ks = smem + stream + stage * STAGE, *Vs = Ks + KB;
-        if (lo_any < kt + KW && hi_any > kt) {
-            const bool full = lo_all <= kt && hi_all >= kt + KW;
-            acc s[NSUB];
+        if constexpr (WQ > 1) {
+            if (more) {
+                issue(next, kpool, buf0 + (stage ^ 1) * STAGE);
+                issue(next, vpool, buf0 + (stage ^ 1) * STAGE + KB);
+                wait_step<2 * NI>();
+            } else {
+                wait_step<0>();
+            }
+            block_barrier();
+        } else {
+            wait_step<NI>();  // K; V may still be on its way
+        }
+        acc s[NSUB];
+        float unit = sc;  // of s, in log2 units
+        if (seen) {
 #pragma unroll
             for (int j = 0; j < NSUB; ++j) {
 #pragma unroll
@@ -444,14 +500,25 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
                     if constexpr (kSplit) s[j] = Mx<C>::mm(k, ql[c], s[j]);
                 }
             }
-            float unit = sc;  // of s, in log2 units
+        }
+        if constexpr (WQ == 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
+            if (more) {
+                issue(next, kpool, buf0);
+                wait_step<NI>();  // V
+            } else {
+                wait_step<0>();
+            }
+        }
+        if (seen) {
+            const bool full = lo_all <= kt && hi_all >= kt + KW;
             if (capped || biased || sc == 0.f) {  // (a scale of zero times a masked score is no number)
 #pragma unroll
                 for (int j = 0; j < NSUB; ++j)
 #pragma unroll
                     for (int i = 0; i < AV; ++i) {
                         float z = s[j][i] * sc;
-                        if (capped) z = cap2 * tanh_f(z);
+                        if (capped) z = cap2 * tanh_f<kSplit>(z);
                         if (biased) z -= slope * fabsf(float(pos - kt - key_in(j, i)));
                         s[j][i] = z;
                     }
@@ -492,16 +559,12 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
                     sum += p[e];
                 }
                 if constexpr (kSplit) {
-                    u32x4 h4, l4;
+                    // (no asm here: what it writes, the compiler would not keep apart from a product that still reads)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        uint32_t hi, lo;
-                        split_f16x2(p[2 * e], p[2 * e + 1], hi, lo);
-                        h4[e] = hi;
-                        l4[e] = lo;
+                    for (int e = 0; e < 8; ++e) {
+                        ph[e] = _Float16(p[e]);
+                        pl[e] = _Float16(p[e] - float(ph[e]));
                     }
-                    ph = __builtin_bit_cast(v8, h4);
-                    pl = __builtin_bit_cast(v8, l4);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ph[e] = C(p[e]);
@@ -522,15 +585,15 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
             // A value that is not finite may stand at a key that only some rows see: 0 times it would reach the others
             bool wild = false;
             if (!full) {
+                u16x8 top = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < KB / 1024; ++i) {
-                    const u16x8 x = *reinterpret_cast<const u16x8 *>(Vs + i * 1024 + lane * 16);
+                for (int i = 0; i < KB / 1024; ++i)
+                    top = __builtin_elementwise_max(top, *reinterpret_cast<const u16x8 *>(Vs + i * 1024 + lane * 16) & uint16_t(0x7FFF));
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) wild |= (x[e] & Mx<C>::kExp) == Mx<C>::kExp;
-                }
+                for (int e = 0; e < 8; ++e) wild |= top[e] >= Mx<C>::kExp;
                 wild = __any(wild);
             }
-            if (!wild) {
+            if (__builtin_expect(!wild, 1)) {
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     v8 ph, pl;
@@ -542,45 +605,52 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
                         if constexpr (kSplit) o[d] = Mx<C>::mm(v, pl, o[d]);
                     }
                 }
-            } else {  // finite values as above; rows that see one that is not become NaN there
-#pragma unroll 1
-                for (int d = 0; d < ND; ++d) {
-                    acc hit, od;
+            } else {  // the finite ones as above; a row that sees one that is not becomes NaN there
+                int32_t kt_ = kt - see.begin;
+                asm volatile("" : "+v"(kt_));  // (the mask's comparisons anew, not kept since then)
 #pragma unroll
-                    for (int i = 0; i < AV; ++i) hit[i] = od[i] = 0.f;
+                for (int c = 0; c < NC; ++c) {
+                    v8 ph, pl;
+                    l += weights(c, ph, pl);
+                    u16x8 eye;
 #pragma unroll
-                    for (int c = 0; c < NC; ++c) {
-                        u16x8 v = __builtin_bit_cast(u16x8, v_at(c, d)), w, seen;
+                    for (int e = 0; e < 8; ++e) {
+                        const int key = NQ == 32 ? key_in(c / 2, (8 * c + e) & 15) : key_in(2 * c + e / 4, e & 3);
+                        eye[e] = uint32_t(kt_ + key) < see_n ? Mx<C>::kOne : 0;
+                    }
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        u16x8 v = __builtin_bit_cast(u16x8, v_at(c, d)), w;
 #pragma unroll
                         for (int e = 0; e < 8; ++e) {
                             const bool out = (v[e] & Mx<C>::kExp) == Mx<C>::kExp;
                             w[e] = out ? Mx<C>::kOne : 0;
                             v[e] = out ? 0 : v[e];
-                            const int key = kt + (NQ == 32 ? key_in(c / 2, (8 * c + e) & 15) : key_in(2 * c + e / 4, e & 3));
-                            seen[e] = uint32_t(key - see.begin) < see_n ? Mx<C>::kOne : 0;
                         }
-                        v8 ph, pl;
-                        const float sum = weights(c, ph, pl);
-                        l += d == 0 ? sum : 0.f;
-                        od = Mx<C>::mm(__builtin_bit_cast(v8, v), ph, od);
-                        if constexpr (kSplit) od = Mx<C>::mm(__builtin_bit_cast(v8, v), pl, od);
-                        hit = Mx<C>::mm(__builtin_bit_cast(v8, w), __builtin_bit_cast(v8, seen), hit);
+                        o[d] = Mx<C>::mm(__builtin_bit_cast(v8, v), ph, o[d]);
+                        if constexpr (kSplit) o[d] = Mx<C>::mm(__builtin_bit_cast(v8, v), pl, o[d]);
+                        acc hit;
+#pragma unroll
+                        for (int i = 0; i < AV; ++i) hit[i] = 0.f;
+                        hit = Mx<C>::mm(__builtin_bit_cast(v8, w), __builtin_bit_cast(v8, eye), hit);
+#pragma unroll
+                        for (int i = 0; i < AV; ++i) o[d][i] += hit[i] > 0.f ? __builtin_nanf("") : 0.f;
                     }
-#pragma unroll
-                    for (int x = 0; x < ND; ++x)
-#pragma unroll
-                        for (int i = 0; i < AV; ++i)
-                            if (x == d) o[x][i] += hit[i] > 0.f ? __builtin_nanf("") : od[i];
                 }
             }
         }
-        if constexpr (WQ > 1) read_barrier();
+        if constexpr (WQ > 1) {
+            read_barrier();
+        } else if (more) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
+            issue(next, vpool, buf0 + KB);
+        }
     }
     raise_status(a.status, bad_page, kStatusBadPage);
     l = rows_sum<NQ>(l);
 
     T *out = static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * hd;
-    const int64_t part = (int64_t(row) * a.heads + head) * a.slots + slot0 + split;
+    const int64_t part = (int64_t(row) * a.heads + head) * a.slots + (GROUPS ? 0 : a.gsplits) + split;
     if constexpr (WK == 1) {
         if (!valid) return;
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
@@ -599,7 +669,7 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
                 else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
             }
     } else {
-        // the waves' parts: maxima and sums, then every wave's rows scaled to the common maximum, added in wave order
+        // the waves' parts side by side in LDS, then every lane adds its 4 dims of a row, in wave order
         constexpr int LDO = HDP + 4;
         float *sm = reinterpret_cast<float *>(smem), *so = sm + 2 * WK * NQ;
         wait_step<0>();
@@ -608,24 +678,24 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
             sm[wk * NQ + col] = m;
             sm[(WK + wk) * NQ + col] = l;
         }
-        wait_step<0>();
-        block_barrier();
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < WK; ++w) M = fmaxf(M, sm[w * NQ + col]);
-#pragma unroll
-        for (int w = 0; w < WK; ++w) L += sm[w * NQ + col] == -INFINITY ? 0.f : exp2_fast(sm[w * NQ + col] - M) * sm[(WK + w) * NQ + col];
-        const float f = m == -INFINITY ? 0.f : exp2_fast(m - M);
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int i = 0; i < AV; i += 4) {
                 const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
-                *reinterpret_cast<f32x4 *>(so + (wk * NQ + col) * LDO + e) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]} * f;
+                *reinterpret_cast<f32x4 *>(so + (wk * NQ + col) * LDO + e) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
             }
         wait_step<0>();
         block_barrier();
         if (!valid) return;
+        float M = -INFINITY, L = 0.f, f[WK];
+#pragma unroll
+        for (int w = 0; w < WK; ++w) M = fmaxf(M, f[w] = sm[w * NQ + col]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+            f[w] = f[w] == -INFINITY ? 0.f : exp2_fast(f[w] - M);
+            L += f[w] * sm[(WK + w) * NQ + col];
+        }
         const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
         if (!whole && wave == 0 && lh == 0) {
             a.ml[2 * part] = M;
@@ -635,41 +705,77 @@ __global__ __launch_bounds__(256, WQ == 4 ? 2 : 1) void k_paged_attn(PagedAttnAr
         for (int e = 4 * (wave * (64 / NQ) + lh); e < hd; e += 4 * 256 / NQ) {
             f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < WK; ++w) x += *reinterpret_cast<const f32x4 *>(so + (w * NQ + col) * LDO + e);
+            for (int w = 0; w < WK; ++w) x += *reinterpret_cast<const f32x4 *>(so + (w * NQ + col) * LDO + e) * f[w];
             if (whole) store4(out + e, x * inv);
             else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
         }
     }
 }
 
+// The tiles of the groups' shared keys (GN query rows a wave, GW waves beside each other; 0: no groups), then those of the
+// sequences' own: one launch, so that neither waits for the other.
+template <class T, class C, int HDP, int GN, int GW, int SN, int SW>
+__global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnArgs a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    int id = blockIdx.x;
+    if constexpr (GN > 0) {
+        const int n = a.gtiles * a.gsplits * a.c.kv_heads;
+        if (id < n) {
+            attn_tile<T, C, HDP, GN, GW, true>(a, id, smem);
+            return;
+        }
+        id -= n;
+    }
+    attn_tile<T, C, HDP, SN, SW, false>(a, id, smem);
+}
+
 // The parts of rows whose keys went in several runs, or partly with a group: M = their largest maximum, sums and outputs scaled
-// by 2^(max - M) and added in slot order. grid x = rows x ceil(heads / 8), block 256: 32 lanes a head, 4 dims each.
+// by 2^(max - M) and added in slot order. desc[row] (0: written already) is the number of a group's parts and, 16 bits up, of
+// the sequence's own. grid x = rows x ceil(heads / 8), block 256: 32 lanes a head, 4 dims each. One round trip finds
+// desc and every slot's maximum and sum (one slot a lane, as many as there are), the next the outputs.
 template <class T>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
     const int hb = (a.heads + 7) / 8, row = int(blockIdx.x) / hb, head = int(blockIdx.x) % hb * 8 + int(threadIdx.x) / 32;
-    const int e = 4 * (int(threadIdx.x) % 32);
-    const int32_t s = find_seq(a.b, row);
-    if (s < 0) return;
-    const Segment seg = seq_segment(a.b, a.p, a.c.shift, s);
-    const int32_t grp = group_of(a.p, s);
-    const int32_t gn = grp >= 0 ? runs_of(0, clamp_i32(a.p.len[grp], 0, a.b.page_ld << a.c.shift), a.gsplits, a.gleast).count : 0;
-    const int32_t sn = runs_of(seg.key0, seg.key1, a.ssplits, a.sleast).count;
-    if (gn == 0 && sn <= 1) return;  // written by its only run
-    if (head >= a.heads || e >= a.c.hd) return;
-    const int64_t base = (int64_t(row) * a.heads + head) * a.slots;
-    auto slot = [&](int i) { return base + (i < gn ? i : a.gsplits + i - gn); };
-    float M = -INFINITY;
-    for (int i = 0; i < gn + sn; ++i) M = fmaxf(M, a.ml[2 * slot(i)]);
-    float L = 0.f;
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < gn + sn; ++i) {
-        const int64_t at = slot(i);
-        const float mi = a.ml[2 * at], li = a.ml[2 * at + 1];
-        const f32x4 oi = *reinterpret_cast<const f32x4 *>(a.po + at * a.c.hd + e);
-        const float f = mi == -INFINITY ? 0.f : exp2_fast(mi - M);
-        L += f * li;
-        x += oi * f;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, e = 4 * l32;
+    const bool on = head < a.heads;
+    const int64_t base = (int64_t(row) * a.heads + (on ? head : 0)) * a.slots;
+    const int32_t r0 = a.b.row_start[0], r1 = a.b.row_start[a.b.seqs], desc = a.desc[row];
+    float mi[2], li[2];  // slots l32 and 32 + l32
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int64_t at = base + min(32 * k + l32, a.slots - 1);
+        mi[k] = a.ml[2 * at];
+        li[k] = a.ml[2 * at + 1];
     }
+    if (row < r0 || row >= r1 || desc == 0) return;
+    const int gn = min(desc & 0xFFFF, a.gsplits), sn = min(desc >> 16, a.ssplits);
+    auto used = [&](int i) { return i < gn || (i >= a.gsplits && i < a.gsplits + sn); };
+    float M = -INFINITY, w[2], L = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        mi[k] = used(32 * k + l32) ? mi[k] : -INFINITY;
+        M = fmaxf(M, mi[k]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        w[k] = mi[k] == -INFINITY ? 0.f : exp2_fast(mi[k] - M);
+        L += used(32 * k + l32) ? w[k] * li[k] : 0.f;  // (a slot that no block wrote holds anything)
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    const float *po = a.po + base * a.c.hd + (e < a.c.hd ? e : 0);
+    auto add = [&](int i) {
+        const float f = __shfl(w[i >> 5], (lane & 32) + (i & 31), 64);
+        x += *reinterpret_cast<const f32x4 *>(po + int64_t(i) * a.c.hd) * f;
+    };
+#pragma unroll 4
+    for (int i = 0; i < gn; ++i) add(i);
+#pragma unroll 4
+    for (int i = 0; i < sn; ++i) add(a.gsplits + i);
+    if (!on || e >= a.c.hd) return;
     const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
     store4(static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * a.c.hd + e, x * inv);
 }

@@ -338,16 +338,17 @@ struct PagedAttnArgs {
     int32_t heads, window;
     float scale, cap;
     int32_t *status;
-    // the parts of rows whose keys go in several runs: slots of a (row, head), a group's gsplits then a sequence's ssplits; ml
-    // (max, sum) and po [head_dim] of each, behind each other in one workspace
+    // the launch (PagedPlan), and the parts of rows whose keys go in several runs: slots of a (row, head), a group's gsplits then a
+    // sequence's ssplits; ml (max, sum) and po [head_dim] of each, desc of each row, behind each other in one workspace
     float *ml, *po;
-    int32_t slots, gsplits, ssplits, gleast, sleast;
+    int32_t *desc;
+    int32_t slots, gsplits, ssplits, gleast, sleast, gtiles, stiles, direct;
 };
 // Where the attention's launches come from: tiles and splits by the batch's bounds, and the floats of its workspace.
 struct PagedPlan {
     int32_t stile, gtile;    // query rows of a tile of a sequence, of a group (0: no groups)
     int32_t stiles, gtiles;  // at most so many tiles
-    bool direct;             // tile i is sequence i
+    int32_t direct;          // tile i is sequence i
     int32_t gsplits, ssplits, gleast, sleast, slots;
     int64_t ws_floats;
 };

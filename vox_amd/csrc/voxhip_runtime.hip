@@ -3944,6 +3944,7 @@ PagedKv paged_kv(const voxhip_paged_kv *kv) {
     need(kv->page_stride > 0 && kv->head_stride > 0 && kv->pos_stride >= kv->head_dim && kv->page_stride % 8 == 0 && kv->head_stride % 8 == 0 &&
              kv->pos_stride % 8 == 0,
          "strides are positive multiples of 8 elements, pos_stride at least head_dim");
+    need(kv->pos_stride <= (1 << 26), "pos_stride is too large");  // 8 of them stay in 32 bits of bytes
     // one page of one head, all heads and all pages lie apart: positions inside heads or heads inside positions, both inside a page
     const int64_t in_head = int64_t(kv->page_size - 1) * kv->pos_stride + kv->head_dim, in_pos = int64_t(kv->kv_heads - 1) * kv->head_stride + kv->head_dim;
     need(kv->kv_heads == 1 || kv->head_stride >= in_head || (kv->head_stride >= kv->head_dim && kv->pos_stride >= in_pos), "heads and positions of a page overlap");
