@@ -115,13 +115,20 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
-// Matrix products of the cache's type: c += a b, columns of b in the lanes' low bits, the K elements of a lane neighbours.
+// Of the cache's type: the sum of 8 values onto c in 32 bits; matrix products: c += a b, columns of b in the lanes' low bits, the K elements of a lane neighbours.
 template <class C>
 struct Mx;
 template <>
 struct Mx<_Float16> {
     typedef f16x8 v8;
     static constexpr uint16_t kExp = 0x7C00, kOne = 0x3C00;
+    static VH_DEV float sum(v8 a, float c) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 one = {1, 1};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2(f16x2{a[i], a[i + 1]}, one, c, false);
+        return c;
+    }
     static VH_DEV f32x16 mm(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static VH_DEV f32x4 mm(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
@@ -129,6 +136,13 @@ template <>
 struct Mx<__bf16> {
     typedef bf16x8 v8;
     static constexpr uint16_t kExp = 0x7F80, kOne = 0x3F80;
+    static VH_DEV float sum(v8 a, float c) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        const bf16x2 one = {__bf16(1.f), __bf16(1.f)};
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) c = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{a[i], a[i + 1]}, one, c, false);
+        return c;
+    }
     static VH_DEV f32x16 mm(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static VH_DEV f32x4 mm(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
@@ -257,7 +271,6 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     constexpr int ND = HDP / NQ;                                                  // O^T products
     constexpr int NC = KW / KD;                                                   // P^T operands
     constexpr float kUp = std::is_same<C, __bf16>::value ? 0.f : 6.f, kLag = 8.f;
-    static_assert(NI >= 1 && (NI % 2 == 0 || R == 8), "the swizzle's parity is the DMA's");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
     const int wq = wave % WQ, wk = wave / WQ, col = lane % NQ, lh = lane / NQ;  // lh: which rows of a product this lane holds
     const int G = a.c.kv_heads, group = a.heads / G, hd = a.c.hd;
@@ -323,6 +336,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     }
     const float slope_raw = a.slopes ? a.slopes[head] : 0.f;
     int32_t pos, lo_any, hi_any, lo_all, hi_all;  // of the wave's rows: the keys that any sees, and those that all see
+    int32_t lo_blk, hi_blk;                       // of the block's rows: those that all see
     int32_t kb = run.begin, ke = run.end;         // the block's keys
     Span see;
     if constexpr (GROUPS) {
@@ -343,8 +357,14 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         lo_any = run.begin;
         hi_any = run.end;
         const bool all = __all(!valid || (see.begin <= run.begin && see.end >= run.end));
-        lo_all = all ? run.begin : INT32_MAX;
-        hi_all = run.end;
+        lo_all = lo_blk = all ? run.begin : INT32_MAX;
+        hi_all = hi_blk = run.end;
+        if constexpr (WQ > 1) {
+            __shared__ int32_t least[4];
+            if (lane == 0) least[wave] = lo_all;
+            read_barrier();
+            lo_blk = max(max(least[0], least[1]), max(least[2], least[3]));
+        }
     } else {
         // a sequence's rows see no less at either end the later they stand
         const int32_t pf = a.prefix ? a.prefix[seg_id] : 0, len = seg.key1, before = len - seg.rows;
@@ -359,6 +379,8 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         hi_any = min(last.end, run.end);
         lo_all = max(last.begin, run.begin);
         hi_all = min(first.end, run.end);
+        lo_blk = WQ > 1 ? max(b1.begin, run.begin) : lo_all;
+        hi_blk = WQ > 1 ? min(b0.end, run.end) : hi_all;
     }
     see.begin = max(see.begin, run.begin);
     see.end = valid ? min(see.end, run.end) : 0;
@@ -372,15 +394,22 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const float sc = fabsf(a.scale) * (capped ? 1.f / a.cap : kLog2e), cap2 = a.cap * kLog2e;
     const float slope = slope_raw * kLog2e;
 
-    // DMA: this lane's key of R and piece of CPR, by the DMA's parity where the swizzle needs it
+    // DMA: this lane's key of R and piece of CPR; where the swizzle needs more of the key than its place in the DMA, by the DMA's
+    // number. K: piece ^ key, so that 16 keys' reads of one piece meet nowhere; V: by pairs of pieces, which its blocks of 16
+    // dims are.
+    constexpr int VK = PITCH == 256 ? 4 : 2;
+    static_assert(NI % VK == 0, "the swizzle goes by the DMA's number");
     const int rin = lane / CPR, piece = lane % CPR;
-    uint32_t voff[2];
-    bool vin[2];
+    uint32_t koff[VK], voff[VK];
+    uint32_t kin = 0, vin = 0;  // bit n: the piece lies inside head_dim
 #pragma unroll
-    for (int par = 0; par < 2; ++par) {
-        const int p = PITCH == 256 ? piece ^ (((4 * par + rin) & 7) << 1) : piece ^ (((rin >> 1) & 3) << 1);
-        voff[par] = (uint32_t(rin) * uint32_t(a.c.pos_stride) + 8 * p) * 2;
-        vin[par] = 8 * p < hd;
+    for (int n = 0; n < VK; ++n) {
+        const int kp = piece ^ (PITCH == 256 ? 4 * n + rin : 4 * n + (rin >> 1));
+        const int vp = piece ^ (PITCH == 256 ? ((4 * n + rin) & 7) << 1 : ((rin >> 1) & 3) << 1);
+        koff[n] = (uint32_t(rin) * uint32_t(a.c.pos_stride) + 8 * kp) * 2;
+        voff[n] = (uint32_t(rin) * uint32_t(a.c.pos_stride) + 8 * vp) * 2;
+        kin |= uint32_t(8 * kp < hd) << n;
+        vin |= uint32_t(8 * vp < hd) << n;
     }
     const int32_t *tab = a.b.table + int64_t(seg.seq0) * a.b.page_ld;
     const int32_t last_page = run.end > run.begin ? (run.end - 1) >> a.c.shift : 0, first_page = run.begin >> a.c.shift;
@@ -393,7 +422,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const int64_t page_bytes = a.c.page_stride * 2;
     const uint32_t pos_bytes = uint32_t(a.c.pos_stride) * 2;
     const int shift = a.c.shift;
-    auto issue = [&](int32_t kt, const uint8_t *from, uint32_t buf) {
+    auto issue = [&](int32_t kt, const uint8_t *from, const uint32_t (&off)[VK], uint32_t inside, uint32_t buf) {
         const int32_t i0 = max(kt >> shift, first_page), i1 = min((kt + KW - 1) >> shift, last_page);
         if (i0 < pbase || i1 >= pbase + 64) {
             pbase = i0;
@@ -409,17 +438,17 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
             for (int n = 0; n < NI; ++n) {
                 const int i = wq * NI + n;
                 const int32_t key = kt + R * i;
-                dma_off16(from + at(__builtin_amdgcn_readlane(pg, (key >> shift) - pbase), key), voff[n & 1], buf + i * 1024);
+                dma_off16(from + at(__builtin_amdgcn_readlane(pg, (key >> shift) - pbase), key), off[n % VK], buf + i * 1024);
             }
         } else {
-#pragma unroll 2
+#pragma unroll
             for (int n = 0; n < NI; ++n) {
                 const int i = wq * NI + n;
                 const int32_t key = kt + R * i, mine = key + rin;
                 const int32_t page = __builtin_amdgcn_readlane(pg, (min(max(key >> shift, i0), i1) - pbase) & 63);
-                const bool in = page >= 0 && vin[n & 1] && mine >= run.begin && mine < run.end;
+                const bool in = page >= 0 && (inside >> (n % VK) & 1) && mine >= run.begin && mine < run.end;
                 const uint8_t *zero = reinterpret_cast<const uint8_t *>(kZero16);
-                dma_lane16(in ? from + at(page, key) + voff[n & 1] : zero, buf + i * 1024);
+                dma_lane16(in ? from + at(page, key) + off[n % VK] : zero, buf + i * 1024);
             }
         }
     };
@@ -428,8 +457,8 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const uint32_t stream = uint32_t(wk) * STAGES * STAGE, buf0 = lds0 + stream;
     const int32_t k_first = kb + wk * KW;
     if (k_first < ke) {
-        issue(k_first, kpool, buf0);
-        issue(k_first, vpool, buf0 + KB);
+        issue(k_first, kpool, koff, kin, buf0);
+        issue(k_first, vpool, voff, vin, buf0 + KB);
     }
 
     // queries as the second operand of S^T: column col, K elements 8 lh .. of every product. A negative scale turns them
@@ -463,7 +492,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     float m = -INFINITY, l = 0.f;  // m: the running maximum in log2 units; l: this lane's share of the sum
     // LDS addresses: K operand, key col (+ NQ j), piece (KD / 8) c + lh; V^T operand, key 4 (lane / 16 or lh) + lane / 4 % 4,
     // dims 4 (lane % 4) of 16 (and the upper 16 of 32 for odd lane / 16)
-    const int ksw = PITCH == 256 ? (col & 7) << 1 : ((col >> 1) & 3) << 1;
+    const int ksw = PITCH == 256 ? col & 15 : (col >> 1) & 7;
     const int vi = lane & 15, vkey = (NQ == 32 ? 4 * lh : 4 * (lane >> 4)) + (vi >> 2), vd = (NQ == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((vi & 3) >> 1);
     const int vsw = PITCH == 256 ? (vkey & 7) << 1 : ((vkey >> 1) & 3) << 1;
     // value i of S^T product j: its key in the tile
@@ -476,8 +505,8 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         const uint8_t *Ks = smem + stream + stage * STAGE, *Vs = Ks + KB;
         if constexpr (WQ > 1) {
             if (more) {
-                issue(next, kpool, buf0 + (stage ^ 1) * STAGE);
-                issue(next, vpool, buf0 + (stage ^ 1) * STAGE + KB);
+                issue(next, kpool, koff, kin, buf0 + (stage ^ 1) * STAGE);
+                issue(next, vpool, voff, vin, buf0 + (stage ^ 1) * STAGE + KB);
                 wait_step<2 * NI>();
             } else {
                 wait_step<0>();
@@ -504,10 +533,67 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         if constexpr (WQ == 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K has been read
             if (more) {
-                issue(next, kpool, buf0);
+                issue(next, kpool, koff, kin, buf0);
                 wait_step<NI>();  // V
             } else {
                 wait_step<0>();
+            }
+        }
+        auto v_at = [&](int c, int d) {
+            // keys KD c + (4 neighbours, then 4 neighbours 8 or 16 on), dims NQ d ..
+            const uint8_t *at = Vs + (KD * c + vkey) * PITCH + (((NQ / 8 * d + vd) ^ vsw) << 4) + (vi & 1) * 8;
+            union {
+                s16x4 half[2];
+                v8 whole;
+            } r;
+            r.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
+            r.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + (NQ == 32 ? 8 : 16) * PITCH));
+            return r.whole;
+        };
+        // A value that is not finite may stand at a key that only some rows see, and 0 times it would reach the others. Then a
+        // row that sees one becomes NaN in its place, and V goes on without them. All waves of a shared tile look at the same
+        // values, and so decide alike.
+        if (WQ > 1 ? !(lo_blk <= kt && hi_blk >= kt + KW) : seen && !(lo_all <= kt && hi_all >= kt + KW)) {
+            u16x8 top = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KB / 1024; ++i)
+                top = __builtin_elementwise_max(top, *reinterpret_cast<const u16x8 *>(Vs + i * 1024 + lane * 16) & uint16_t(0x7FFF));
+            bool wild = false;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) wild |= top[e] >= Mx<C>::kExp;
+            if (__builtin_expect(__any(wild), 0)) {
+                if (seen) {
+#pragma unroll 1
+                    for (int c = 0; c < NC; ++c) {
+                        u16x8 eye;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int key = KD * c + (NQ == 32 ? (e & 3) + 8 * (e >> 2) : (e & 3) + 16 * (e >> 2)) + 4 * lh;
+                            eye[e] = uint32_t(kt + key - see.begin) < see_n ? Mx<C>::kOne : 0;
+                        }
+#pragma unroll
+                        for (int d = 0; d < ND; ++d) {
+                            u16x8 w = __builtin_bit_cast(u16x8, v_at(c, d));
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) w[e] = (w[e] & 0x7FFF) >= Mx<C>::kExp ? Mx<C>::kOne : 0;
+                            acc hit;
+#pragma unroll
+                            for (int i = 0; i < AV; ++i) hit[i] = 0.f;
+                            hit = Mx<C>::mm(__builtin_bit_cast(v8, w), __builtin_bit_cast(v8, eye), hit);
+#pragma unroll
+                            for (int i = 0; i < AV; ++i) o[d][i] = hit[i] > 0.f ? __builtin_nanf("") : o[d][i];
+                        }
+                    }
+                }
+                if constexpr (WQ > 1) read_barrier();
+                for (int i = wq; i < KB / 1024; i += WQ) {
+                    u16x8 *at = reinterpret_cast<u16x8 *>(smem + stream + stage * STAGE + KB + i * 1024 + lane * 16);
+                    u16x8 x = *at;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = (x[e] & 0x7FFF) >= Mx<C>::kExp ? 0 : x[e];
+                    *at = x;
+                }
+                if constexpr (WQ > 1) read_barrier();
             }
         }
         if (seen) {
@@ -556,7 +642,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
                     // 32 x 32: 8 neighbouring registers; 16 x 16: the 4 of two products
                     const float x = NQ == 32 ? s[c / 2][(8 * c + e) & 15] : s[2 * c + e / 4][e & 3];
                     p[e] = exp2_fast(fmaf(x, unit, add));
-                    sum += p[e];
+                    if constexpr (kSplit) sum += p[e];
                 }
                 if constexpr (kSplit) {
                     // (no asm here: what it writes, the compiler would not keep apart from a product that still reads)
@@ -568,74 +654,19 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
                 } else {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) ph[e] = C(p[e]);
+                    sum = Mx<C>::sum(ph, sum);  // of the rounded weights, which V meets
                 }
                 return sum;
             };
-            auto v_at = [&](int c, int d) {
-                // keys KD c + (4 neighbours, then 4 neighbours 8 or 16 on), dims NQ d ..
-                const uint8_t *at = Vs + (KD * c + vkey) * PITCH + (((NQ / 8 * d + vd) ^ vsw) << 4) + (vi & 1) * 8;
-                union {
-                    s16x4 half[2];
-                    v8 whole;
-                } r;
-                r.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
-                r.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + (NQ == 32 ? 8 : 16) * PITCH));
-                return r.whole;
-            };
-            // A value that is not finite may stand at a key that only some rows see: 0 times it would reach the others
-            bool wild = false;
-            if (!full) {
-                u16x8 top = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
-                for (int i = 0; i < KB / 1024; ++i)
-                    top = __builtin_elementwise_max(top, *reinterpret_cast<const u16x8 *>(Vs + i * 1024 + lane * 16) & uint16_t(0x7FFF));
+            for (int c = 0; c < NC; ++c) {
+                v8 ph, pl;
+                l += weights(c, ph, pl);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) wild |= top[e] >= Mx<C>::kExp;
-                wild = __any(wild);
-            }
-            if (__builtin_expect(!wild, 1)) {
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    v8 ph, pl;
-                    l += weights(c, ph, pl);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        const v8 v = v_at(c, d);
-                        o[d] = Mx<C>::mm(v, ph, o[d]);
-                        if constexpr (kSplit) o[d] = Mx<C>::mm(v, pl, o[d]);
-                    }
-                }
-            } else {  // the finite ones as above; a row that sees one that is not becomes NaN there
-                int32_t kt_ = kt - see.begin;
-                asm volatile("" : "+v"(kt_));  // (the mask's comparisons anew, not kept since then)
-#pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    v8 ph, pl;
-                    l += weights(c, ph, pl);
-                    u16x8 eye;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int key = NQ == 32 ? key_in(c / 2, (8 * c + e) & 15) : key_in(2 * c + e / 4, e & 3);
-                        eye[e] = uint32_t(kt_ + key) < see_n ? Mx<C>::kOne : 0;
-                    }
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        u16x8 v = __builtin_bit_cast(u16x8, v_at(c, d)), w;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool out = (v[e] & Mx<C>::kExp) == Mx<C>::kExp;
-                            w[e] = out ? Mx<C>::kOne : 0;
-                            v[e] = out ? 0 : v[e];
-                        }
-                        o[d] = Mx<C>::mm(__builtin_bit_cast(v8, v), ph, o[d]);
-                        if constexpr (kSplit) o[d] = Mx<C>::mm(__builtin_bit_cast(v8, v), pl, o[d]);
-                        acc hit;
-#pragma unroll
-                        for (int i = 0; i < AV; ++i) hit[i] = 0.f;
-                        hit = Mx<C>::mm(__builtin_bit_cast(v8, w), __builtin_bit_cast(v8, eye), hit);
-#pragma unroll
-                        for (int i = 0; i < AV; ++i) o[d][i] += hit[i] > 0.f ? __builtin_nanf("") : 0.f;
-                    }
+                for (int d = 0; d < ND; ++d) {
+                    const v8 v = v_at(c, d);
+                    o[d] = Mx<C>::mm(v, ph, o[d]);
+                    if constexpr (kSplit) o[d] = Mx<C>::mm(v, pl, o[d]);
                 }
             }
         }
@@ -643,7 +674,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
             read_barrier();
         } else if (more) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // V has been read
-            issue(next, vpool, buf0 + KB);
+            issue(next, vpool, voff, vin, buf0 + KB);
         }
     }
     raise_status(a.status, bad_page, kStatusBadPage);
