@@ -72,7 +72,8 @@ def test_append(change, why):
     (dict(at_type=vh.Q4), "rows are"), (dict(at_heads=5), "multiple"), (dict(at_heads=2048), "heads"), (dict(at_q=None), "q is missing"),
     (dict(at_out=None), "out is missing"), (dict(at_ld_q=248), "shorter"), (dict(at_ld_out=260), "multiple of 8"),
     (dict(at_scale=float("inf")), "scale"), (dict(at_cap=-1.0), "cap"), (dict(at_cap=float("nan")), "cap"), (dict(at_window=-1), "window"),
-    (dict(at_slopes=A + 2), "slopes"), (dict(at_prefix=A + 1), "prefix"), (dict(at_out=A + 16), "partly")],
+    (dict(at_slopes=A + 2), "slopes"), (dict(at_prefix=A + 1), "prefix"), (dict(at_out=A + 16), "partly"),
+    (dict(at_heads=1024, b_rows=(1 << 20) + 1), "rows x heads")],
     ids=lambda v: "-".join(v) if isinstance(v, dict) else None)
 def test_attention(change, why):
     kv, b, _, at, sh = parts(**change)

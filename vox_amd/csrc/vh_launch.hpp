@@ -188,7 +188,7 @@ hipError_t launch_acc_fold(float *h, int64_t *acc, int H, hipStream_t s);
 // Paged cache (vh_paged.hpp); type: the rows' WT_F32, WT_F16 (f16 cache) or WT_BF16 (bf16 cache).
 hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s);
 PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_len, int32_t max_shared);
-hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &plan, float *ws, hipStream_t s);
+hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &plan, float *ws, int32_t *count, hipStream_t s);
 
 // Shared-memory opt-in above 64 KiB, once per kernel.
 hipError_t ensure_smem(const void *kernel, size_t bytes);

@@ -20,7 +20,9 @@ hipError_t by_type(int type, F &&f) {
 hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0) return hipErrorInvalidValue;
     const int lph = a.c.hd <= 64 ? 16 : 32, per = 256 / lph;
-    a.blocks = (a.heads + 2 * a.c.kv_heads + per - 1) / per;
+    // turns of heads per row as blocks of their own up to about 2048 blocks (8 a CU), which hide each other's chains of reads
+    const int64_t turns = (a.heads + 2 * a.c.kv_heads + per - 1) / per;
+    a.blocks = int32_t(std::max<int64_t>(1, std::min<int64_t>(turns, 2048 / a.b.rows)));
     const int64_t grid = int64_t(a.b.rows) * a.blocks;
     if (grid > INT32_MAX) return hipErrorInvalidValue;
     a.status = status_word();
@@ -55,7 +57,11 @@ PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_
         p.gsplits = splits_for(std::max<int64_t>(1, q / p.gtile), std::max(max_shared, 1));
     }
     p.slots = p.gsplits + p.ssplits;
-    p.ws_floats = p.gsplits || p.ssplits > 1 ? int64_t(a.b.rows) * a.heads * p.slots * (2 + a.c.hd) + a.b.rows : 0;
+    if (p.gsplits || p.ssplits > 1) {
+        p.parts = int64_t(a.b.rows) * a.heads * p.slots;
+        p.ws_floats = p.parts * (2 + a.c.hd) + a.b.rows;
+        p.counts = p.stile <= 32 && p.gtile <= 32 ? int64_t(a.b.rows) * a.heads : 0;
+    }
     return p;
 }
 
@@ -88,24 +94,25 @@ hipError_t attn_of(const PagedAttnArgs &a, int gtile, int stile, hipStream_t s) 
 }
 }  // namespace
 
-hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &p, float *ws, hipStream_t s) {
-    if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0 || (p.ws_floats && !ws) || p.slots > 64) return hipErrorInvalidValue;
-    const int64_t join = int64_t(a.b.rows) * ((a.heads + 7) / 8);
-    if (join > INT32_MAX) return hipErrorInvalidValue;
+hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &p, float *ws, int32_t *count, hipStream_t s) {
+    if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0 || (p.ws_floats && !ws) || (p.counts && !count) || p.slots > 64)
+        return hipErrorInvalidValue;
+    const int32_t group = a.heads / a.c.kv_heads;
     a.status = status_word();
+    a.magic = uint32_t((uint64_t(1) << 32) / uint64_t(group)) + 1;
     a.slots = p.slots; a.gsplits = p.gsplits; a.ssplits = p.ssplits; a.gleast = p.gleast; a.sleast = p.sleast;
     a.gtiles = p.gtiles; a.stiles = p.stiles; a.direct = p.direct;
-    if (p.ws_floats) {
-        const int64_t parts = int64_t(a.b.rows) * a.heads * p.slots;
-        a.po = ws;  // 16-byte aligned rows first
-        a.ml = ws + parts * a.c.hd;
-        a.desc = reinterpret_cast<int32_t *>(a.ml + 2 * parts);
-    }
+    a.po = ws;  // 16-byte aligned rows first
+    a.ml = ws ? ws + p.parts * a.c.hd : nullptr;
+    a.count = p.counts ? count : nullptr;
+    a.desc = p.ws_floats && !p.counts ? reinterpret_cast<int32_t *>(a.ml + 2 * p.parts) : nullptr;
+    const int64_t join = int64_t(a.b.rows) * ((a.heads + 7) / 8);
+    if (join > INT32_MAX) return hipErrorInvalidValue;
     return by_type(type, [&](auto t, auto c) {
         using T = decltype(t);
         using C = decltype(c);
         const hipError_t e = a.c.hd <= 64 ? attn_of<T, C, 64>(a, p.gtile, p.stile, s) : attn_of<T, C, 128>(a, p.gtile, p.stile, s);
-        if (e != hipSuccess || !p.ws_floats) return e;
+        if (e != hipSuccess || !a.desc) return e;
         return launch(k_paged_join<T>, dim3(unsigned(join)), dim3(256), 0, s, a);
     });
 }

@@ -38,15 +38,17 @@ VH_DEV void store4(T *p, f32x4 v) {
     *reinterpret_cast<t4 *>(p) = t4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
 }
 
-// One head of one row per LPH lanes, 4 neighbouring values a lane; grid x = rows x a.blocks, block 256 (256 / LPH heads). A
+// One head of one row per LPH lanes, 4 neighbouring values a lane, 256 / LPH heads at a time; grid x = rows x a.blocks, block 256:
+// block i of a row takes its heads in turns i, i + a.blocks, ... (one each for a step's few rows, all of them where rows
+// alone fill the chip: a block's chain of dependent reads, not the bytes, is what a row costs). A
 // lane of a rotated head also loads the 4 values its own are paired with (halves: rot / 2 away, in L1 by then;
 // interleaved: among its own), so no value crosses lanes but the norm's sum. Rows behind the last sequence, and rows at
 // negative positions, write nothing.
 template <class T, class C, int LPH>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     const int row = int(blockIdx.x) / a.blocks;
-    const int hh = (int(blockIdx.x) % a.blocks) * (256 / LPH) + int(threadIdx.x) / LPH, e = 4 * (int(threadIdx.x) % LPH);
-    const int hd = a.c.hd, G = a.c.kv_heads;
+    const int e = 4 * (int(threadIdx.x) % LPH);
+    const int hd = a.c.hd, G = a.c.kv_heads, heads = a.heads + 2 * G;
     const int32_t s = find_seq(a.b, row);
     if (s < 0) return;
     const SeqRows sr = seq_rows(a.b, a.c.shift, s);
@@ -57,18 +59,13 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
         raise_status(a.status, true, kStatusBadBatch);
         return;
     }
-    const bool on = hh < a.heads + 2 * G && e < hd;
-    const int hc = on ? hh : 0, ec = on ? e : 0;
-    const bool is_q = hc < a.heads, is_v = hc >= a.heads + G;
-    const T *src = static_cast<const T *>(a.qkv) + int64_t(row) * a.ld_qkv + int64_t(hc) * hd;
-    const float *nw = is_v ? nullptr : is_q ? a.qn : a.kn;
-    const bool turn = a.rope && !is_v && ec < a.rot;
-    const int half = a.rot >> 1;
-    const int pe = !turn || a.interleaved ? ec : ec < half ? ec + half : ec - half;
-    f32x4 x = load4(src + ec), xp = load4(src + pe);
+    const int32_t page = page_of(a.c, a.b.table + int64_t(s) * a.b.page_ld, pos);
+    const T *from = static_cast<const T *>(a.qkv) + int64_t(row) * a.ld_qkv;
+    const int half = a.rot >> 1, ec = e < hd ? e : 0;
+    const bool inside = a.rope && ec < a.rot;
     // (cos, sin) of this lane's pairs: four pairs of the halves, or two of neighbours
     f32x4 cs0 = {1.f, 0.f, 1.f, 0.f}, cs1 = cs0;
-    if (turn) {
+    if (inside) {
         const float *rp = a.rope + int64_t(pos) * a.rot;
         if (a.interleaved) {
             cs0 = *reinterpret_cast<const f32x4 *>(rp + ec);
@@ -78,34 +75,50 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
             cs1 = *reinterpret_cast<const f32x4 *>(r + 4);
         }
     }
-    if (nw) {  // a head's lanes share the branch; every lane of the wave takes part in the sum below
-        const f32x4 w = *reinterpret_cast<const f32x4 *>(nw + ec), wp = *reinterpret_cast<const f32x4 *>(nw + pe);
-        const float ss = group_sum<LPH>(on ? x[0] * x[0] + x[1] * x[1] + (x[2] * x[2] + x[3] * x[3]) : 0.f);
-        const float inv = 1.0f / sqrtf(ss / float(hd) + a.eps);
-        x = w * (x * inv);
-        xp = wp * (xp * inv);
-    }
-    if (!on) return;
-    if (turn) {
-        if (a.interleaved) {
-            x = f32x4{x[0] * cs0[0] - x[1] * cs0[1], x[1] * cs0[0] + x[0] * cs0[1], x[2] * cs0[2] - x[3] * cs0[3],
-                      x[3] * cs0[2] + x[2] * cs0[3]};
-        } else {
-            const f32x4 c = {cs0[0], cs0[2], cs1[0], cs1[2]}, sn = {cs0[1], cs0[3], cs1[1], cs1[3]};
-            x = ec < half ? x * c - xp * sn : x * c + xp * sn;
+    const int pe = !inside || a.interleaved ? ec : ec < half ? ec + half : ec - half;
+    constexpr int PER = 256 / LPH;
+    // the first values of the next turn are loaded during this one
+    auto head_of = [&](int turn) { return (int(blockIdx.x) % a.blocks + turn * a.blocks) * PER + int(threadIdx.x) / LPH; };
+    auto clamped = [&](int hh) { return hh < heads ? hh : heads - 1; };
+    const int turns = ((heads + PER - 1) / PER + a.blocks - 1) / a.blocks;
+    f32x4 nx = load4(from + int64_t(clamped(head_of(0))) * hd + ec), np = load4(from + int64_t(clamped(head_of(0))) * hd + pe);
+    for (int k = 0; k < turns; ++k) {
+        const int hh = head_of(k), hc = clamped(hh);
+        const bool on = hh < heads && e < hd, is_q = hc < a.heads, is_v = hc >= a.heads + G;
+        f32x4 x = nx, xp = np;
+        if (k + 1 < turns) {
+            const T *src = from + int64_t(clamped(head_of(k + 1))) * hd;
+            nx = load4(src + ec);
+            np = load4(src + pe);
         }
+        const float *nw = is_v ? nullptr : is_q ? a.qn : a.kn;
+        if (nw) {  // a head's lanes share the branch
+            const f32x4 w = *reinterpret_cast<const f32x4 *>(nw + ec), wp = *reinterpret_cast<const f32x4 *>(nw + pe);
+            const float ss = group_sum<LPH>(e < hd ? x[0] * x[0] + x[1] * x[1] + (x[2] * x[2] + x[3] * x[3]) : 0.f);
+            const float inv = 1.0f / sqrtf(ss / float(hd) + a.eps);
+            x = w * (x * inv);
+            xp = wp * (xp * inv);
+        }
+        if (!on) continue;
+        if (inside && !is_v) {
+            if (a.interleaved) {
+                x = f32x4{x[0] * cs0[0] - x[1] * cs0[1], x[1] * cs0[0] + x[0] * cs0[1], x[2] * cs0[2] - x[3] * cs0[3],
+                          x[3] * cs0[2] + x[2] * cs0[3]};
+            } else {
+                const f32x4 c = {cs0[0], cs0[2], cs1[0], cs1[2]}, sn = {cs0[1], cs0[3], cs1[1], cs1[3]};
+                x = ec < half ? x * c - xp * sn : x * c + xp * sn;
+            }
+        }
+        if (is_q) {
+            if (a.q) store4(static_cast<T *>(a.q) + int64_t(row) * a.ld_q + int64_t(hc) * hd + ec, x);
+            continue;
+        }
+        if (page < 0) {
+            raise_status(a.status, true, kStatusBadPage);
+            continue;
+        }
+        store4(static_cast<C *>(is_v ? a.c.v : a.c.k) + key_offset(a.c, page, hc - a.heads - (is_v ? G : 0), pos) + ec, x);
     }
-    if (is_q) {
-        if (a.q) store4(static_cast<T *>(a.q) + int64_t(row) * a.ld_q + int64_t(hc) * hd + ec, x);
-        return;
-    }
-    const int32_t page = page_of(a.c, a.b.table + int64_t(s) * a.b.page_ld, pos);
-    if (page < 0) {
-        raise_status(a.status, true, kStatusBadPage);
-        return;
-    }
-    C *dst = static_cast<C *>(is_v ? a.c.v : a.c.k) + key_offset(a.c, page, hc - a.heads - (is_v ? G : 0), pos) + ec;
-    store4(dst, x);
 }
 
 // ------------------------------------------------------------------ attention
@@ -184,21 +197,36 @@ VH_DEV float rows_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// tanh as (1 - t) / (1 + t), t = 2^(-2 |x| log2 e): off by about 2^-24 absolutely. FINE: by about 2^-23 of its value also near
-// zero, where 1 - t cancels: an odd polynomial (Taylor, to x^11) below 0.3. Both are computed and one is taken: no branch.
+// c tanh(x) of x2 = 2 x log2 e. 16-bit rows: c - 2 c / (1 + 2^x2), off by about 2^-23 c. FINE: by about 2^-23 of its value
+// also near zero, where that cancels: an odd polynomial (Taylor, to x^11) below 0.3. Both are computed and one is taken: no
+// branch.
 template <bool FINE>
-VH_DEV float tanh_f(float x) {
-    const float a = fabsf(x), t = exp2_fast(-2.8853900817779268f * a);
-    float big = copysignf((1.f - t) * __builtin_amdgcn_rcpf(1.f + t), x);
+VH_DEV float tanh_f(float x2, float c) {
+    float big = fmaf(-2.f * c, __builtin_amdgcn_rcpf(1.f + exp2_fast(x2)), c);
     if constexpr (!FINE) return big;
-    const float x2 = x * x;
-    float p = fmaf(x2, -1382.0f / 155925.0f, 62.0f / 2835.0f);
-    p = fmaf(x2, p, -17.0f / 315.0f);
-    p = fmaf(x2, p, 2.0f / 15.0f);
-    p = fmaf(x2, p, -1.0f / 3.0f);
-    p = fmaf(x * x2, p, x);
+    const float x = x2 * 0.34657359027997264f, xx = x * x;
+    float p = fmaf(xx, -1382.0f / 155925.0f, 62.0f / 2835.0f);
+    p = fmaf(xx, p, -17.0f / 315.0f);
+    p = fmaf(xx, p, 2.0f / 15.0f);
+    p = fmaf(xx, p, -1.0f / 3.0f);
+    p = c * fmaf(x * xx, p, x);
     asm volatile("" : "+v"(big), "+v"(p));
-    return a < 0.3f ? p : big;
+    return fabsf(x) < 0.3f ? p : big;
+}
+
+// u / d by m = 2^32 / d + 1 (d > 1): at most one too many.
+VH_DEV int32_t div_by(int32_t u, int32_t d, uint32_t m) {
+    const int32_t q = d == 1 ? u : int32_t(__umulhi(uint32_t(u), m));
+    return q - (q * d > u);
+}
+
+// 16 and 8 bytes past the caches that other XCDs do not see (agent scope), for parts that another block joins.
+VH_DEV void put_far(float *p, float a, float b) {
+    __hip_atomic_store(reinterpret_cast<uint64_t *>(p), uint64_t(__float_as_uint(b)) << 32 | __float_as_uint(a), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+VH_DEV float2 get_far(const float *p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return float2{__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32))};
 }
 
 // The group of sequence s (the first that holds it) and its shared keys, or -1 and 0: 64 groups at a time.
@@ -239,6 +267,60 @@ VH_DEV bool find_tile(int32_t n, int32_t t, int32_t group, int32_t tile, F rows_
         t -= __builtin_amdgcn_readlane(sum, 63);
     }
     return false;
+}
+
+// A query row's parts joined by 32 lanes, 4 dims each: M = the largest maximum, sums and outputs scaled by 2^(max - M) and added
+// in slot order. gn parts of its group, then (from slot gsplits on) sn of its own keys.
+template <class T, bool FAR>
+VH_DEV void join_row(const PagedAttnArgs &a, int64_t rh, int32_t gn, int32_t sn) {
+    const int l32 = threadIdx.x & 31, e = 4 * l32, n = gn + sn;
+    const float *ml = a.ml + 2 * rh * a.slots, *po = a.po + rh * a.slots * a.c.hd + (e < a.c.hd ? e : 0);
+    auto slot = [&](int i) { return i < gn ? i : a.gsplits + i - gn; };
+    float m[2], l[2], M = -INFINITY, L = 0.f;  // parts l32 and 32 + l32
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+        if (32 * k + l32 < n) {
+            const float *p = ml + 2 * slot(32 * k + l32);
+            const float2 v = FAR ? get_far(p) : *reinterpret_cast<const float2 *>(p);
+            m[k] = v.x;
+            l[k] = v.y;
+        }
+        M = fmaxf(M, m[k]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        m[k] = m[k] == -INFINITY ? 0.f : exp2_fast(m[k] - M);
+        L += m[k] * l[k];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; i += 8) {  // 8 parts' outputs in flight
+        f32x4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float *p = po + int64_t(slot(min(i + k, n - 1))) * a.c.hd;
+            if constexpr (FAR) {
+                const float2 lo = get_far(p), hi = get_far(p + 2);
+                v[k] = f32x4{lo.x, lo.y, hi.x, hi.y};
+            } else {
+                v[k] = *reinterpret_cast<const f32x4 *>(p);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float f = __shfl(i + k < 32 ? m[0] : m[1], (int(threadIdx.x) & 32) + ((i + k) & 31), 64);
+            if (i + k < n) x += v[k] * f;
+        }
+    }
+    if (e >= a.c.hd) return;
+    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
+    const int64_t row = rh / a.heads;
+    store4(static_cast<T *>(a.out) + row * a.ld_out + (rh - row * a.heads) * a.c.hd + e, x * inv);
 }
 
 // Softmax attention of a tile of query rows over a run of keys, on the matrix cores, transposed: S^T = K Q^T has a query row's
@@ -282,7 +364,8 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const int split = id % splits;
     int32_t t = id / splits, seg_id = t, local = 0, shared = 0;
     Segment seg;
-    bool whole = false;  // a row whose keys are one run is written here, otherwise its parts are joined by k_paged_join
+    bool whole = false;  // rows whose keys are one run are written here, otherwise the last block of a row joins its parts
+    int32_t gruns = 0, pf = 0;
     Runs runs;
     if constexpr (GROUPS) {
         if (!find_tile(a.p.groups, t, group, TILE, [&](int32_t i) { return group_segment(a.b, a.p, a.c.shift, i).rows; }, &seg_id, &local)) return;
@@ -299,6 +382,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
                                     &seg_id, &local))
             return;
         const SeqRows sr = seq_rows(a.b, a.c.shift, seg_id);
+        pf = a.prefix ? a.prefix[seg_id] : 0;
         find_group(a.p, seg_id, a.b.page_ld << a.c.shift, &shared);
         seg = Segment{sr.first, sr.n, seg_id, seg_id + 1, min(shared, sr.len), sr.len, sr.ok};
         runs = runs_of(seg.key0, seg.key1, splits, a.sleast);
@@ -307,20 +391,38 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     raise_status(a.status, threadIdx.x == 0 && (!seg.ok || (!GROUPS && a.direct && qrows > TILE)), kStatusBadBatch);
     if (local * TILE >= qrows) return;
     if constexpr (!GROUPS) {
-        const int32_t gruns = runs_of(0, shared, a.gsplits, a.gleast).count;
+        gruns = runs_of(0, shared, a.gsplits, a.gleast).count;
         whole = gruns == 0 && runs.count <= 1;
-        if (a.desc && split == 0 && g == 0) {  // what the join will find
-            const int32_t first = local * TILE / group, i = first + int(threadIdx.x);
-            if (i * group < min(local * TILE + TILE, qrows) && i < seg.rows) a.desc[seg.row0 + i] = whole ? 0 : gruns | runs.count << 16;
+        if (a.desc && split == 0 && g == 0) {  // what k_paged_join will find
+            const int32_t i = div_by(local * TILE, group, a.magic) + int(threadIdx.x);
+            if (i < seg.rows && i * group < local * TILE + TILE) a.desc[seg.row0 + i] = whole ? 0 : gruns | runs.count << 16;
         }
     }
     if (split >= runs.count && !(whole && split == 0)) return;
     const Span run = runs.count ? run_at(runs, seg.key0, seg.key1, split) : Span{0, 0};
+    auto token = [&](int32_t q) { return div_by(q, group, a.magic); };
+
+    int32_t kb = run.begin, ke = run.end;  // the block's keys
+    if constexpr (!GROUPS) {               // a sequence's rows see no less at either end the later they stand
+        const int32_t before = seg.key1 - seg.rows;
+        kb = max(kb, visible(before + token(local * TILE), seg.key1, pf, a.window).begin);
+        ke = min(ke, visible(before + token(min(local * TILE + TILE, qrows) - 1), seg.key1, pf, a.window).end);
+    }
+    kb = __builtin_amdgcn_readfirstlane(kb & ~(KW * WK - 1));
+    ke = __builtin_amdgcn_readfirstlane(ke);
+    const int32_t k_first = kb + wk * KW;
+    // the pages of 64 table entries from pbase on, lane l that of pbase + l; the first ones on their way before all else
+    const int32_t *tab = a.b.table + int64_t(seg.seq0) * a.b.page_ld;
+    const int shift = a.c.shift;
+    const int32_t last_page = run.end > run.begin ? (run.end - 1) >> shift : 0, first_page = run.begin >> shift;
+    int32_t pg = 0, pbase = max(k_first >> shift, first_page);
+    bool checked = false, bad_page = false;
+    if (k_first < ke) pg = tab[min(pbase + lane, last_page)];
 
     // this lane's query row
     const int32_t u = local * TILE + wq * NQ + col;
     const bool valid = u < qrows;
-    const int32_t tok = valid ? u / group : 0, row = seg.row0 + tok, head = g * group + (valid ? u - tok * group : 0);
+    const int32_t tok = valid ? token(u) : 0, row = seg.row0 + tok, head = g * group + (valid ? u - tok * group : 0);
     // the queries, raw: needed only after the first keys are on their way
     constexpr int NK = HDP / KD;
     u32x4 qraw[NK][kSplit ? 2 : 1];
@@ -337,7 +439,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const float slope_raw = a.slopes ? a.slopes[head] : 0.f;
     int32_t pos, lo_any, hi_any, lo_all, hi_all;  // of the wave's rows: the keys that any sees, and those that all see
     int32_t lo_blk, hi_blk;                       // of the block's rows: those that all see
-    int32_t kb = run.begin, ke = run.end;         // the block's keys
+    int32_t parts = gruns + runs.count;           // of this lane's row
     Span see;
     if constexpr (GROUPS) {
         // the sequence that holds the row: by the guess of one row each, or halving
@@ -354,6 +456,8 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         const SeqRows sr = seq_rows(a.b, a.c.shift, seq);
         pos = sr.len - sr.n + (row - sr.first);
         see = visible(pos, sr.len, a.prefix ? a.prefix[seq] : 0, a.window);
+        gruns = runs.count;
+        parts = gruns + runs_of(min(seg.key1, sr.len), sr.len, a.ssplits, a.sleast).count;
         lo_any = run.begin;
         hi_any = run.end;
         const bool all = __all(!valid || (see.begin <= run.begin && see.end >= run.end));
@@ -366,15 +470,11 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
             lo_blk = max(max(least[0], least[1]), max(least[2], least[3]));
         }
     } else {
-        // a sequence's rows see no less at either end the later they stand
-        const int32_t pf = a.prefix ? a.prefix[seg_id] : 0, len = seg.key1, before = len - seg.rows;
+        const int32_t len = seg.key1, before = len - seg.rows, w0 = local * TILE + wq * NQ;
         pos = before + tok;
         see = visible(pos, len, pf, a.window);
-        auto at = [&](int32_t q) { return visible(before + min(q, qrows - 1) / group, len, pf, a.window); };
-        const int32_t w0 = local * TILE + wq * NQ;
+        auto at = [&](int32_t q) { return visible(before + token(min(q, qrows - 1)), len, pf, a.window); };
         const Span b0 = at(local * TILE), b1 = at(local * TILE + TILE - 1), first = at(w0), last = at(w0 + NQ - 1);
-        kb = max(kb, b0.begin);
-        ke = min(ke, b1.end);
         lo_any = w0 < qrows ? max(first.begin, run.begin) : INT32_MAX;
         hi_any = min(last.end, run.end);
         lo_all = max(last.begin, run.begin);
@@ -391,7 +491,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
 
     constexpr float kLog2e = 1.44269504088896341f;
     const bool capped = a.cap > 0.f, biased = a.slopes != nullptr;
-    const float sc = fabsf(a.scale) * (capped ? 1.f / a.cap : kLog2e), cap2 = a.cap * kLog2e;
+    const float sc = fabsf(a.scale) * kLog2e * (capped ? 2.f / a.cap : 1.f), cap2 = a.cap * kLog2e;  // capped: 2 x log2 e of tanh(x)
     const float slope = slope_raw * kLog2e;
 
     // DMA: this lane's key of R and piece of CPR; where the swizzle needs more of the key than its place in the DMA, by the DMA's
@@ -411,26 +511,23 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         kin |= uint32_t(8 * kp < hd) << n;
         vin |= uint32_t(8 * vp < hd) << n;
     }
-    const int32_t *tab = a.b.table + int64_t(seg.seq0) * a.b.page_ld;
-    const int32_t last_page = run.end > run.begin ? (run.end - 1) >> a.c.shift : 0, first_page = run.begin >> a.c.shift;
-    int32_t pg = -1, pbase = -64;  // lane l: the page of table entry pbase + l
-    bool bad_page = false;
     // K (or V, by its pool's first byte of this kv head) of the keys kt .. kt + KW - 1 to buf. A tile inside the run, of whole
     // pitches and pages of the pool, takes its addresses from scalars alone; otherwise lanes without a key read zeros.
     const uint8_t *const kpool = static_cast<const uint8_t *>(a.c.k) + int64_t(g) * a.c.head_stride * 2;
     const uint8_t *const vpool = static_cast<const uint8_t *>(a.c.v) + int64_t(g) * a.c.head_stride * 2;
     const int64_t page_bytes = a.c.page_stride * 2;
     const uint32_t pos_bytes = uint32_t(a.c.pos_stride) * 2;
-    const int shift = a.c.shift;
     auto issue = [&](int32_t kt, const uint8_t *from, const uint32_t (&off)[VK], uint32_t inside, uint32_t buf) {
         const int32_t i0 = max(kt >> shift, first_page), i1 = min((kt + KW - 1) >> shift, last_page);
-        if (i0 < pbase || i1 >= pbase + 64) {
+        if (i1 >= pbase + 64) {
             pbase = i0;
-            const int32_t i = i0 + lane;
-            const bool in = i <= last_page;
-            const int32_t e = in ? tab[i] : -1;
-            pg = uint32_t(e) < uint32_t(a.c.pages) ? e : -1;
-            bad_page |= __any(in && pg < 0);
+            pg = tab[min(i0 + lane, last_page)];
+            checked = false;
+        }
+        if (!checked) {
+            pg = uint32_t(pg) < uint32_t(a.c.pages) ? pg : -1;
+            bad_page |= __any(pg < 0);
+            checked = true;
         }
         auto at = [&](int32_t page, int32_t key) { return int64_t(page) * page_bytes + int64_t(uint64_t(key & ((1 << shift) - 1)) * pos_bytes); };
         if (hd == PITCH / 2 && !bad_page && kt >= run.begin && kt + KW <= run.end) {
@@ -455,7 +552,6 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     // WQ = 4: two stages of K and V, the next tile on its way during this one. WQ = 1: one buffer each, refilled as soon as the
     // wave has read it: K's during the softmax and V's product, V's during the next K's.
     const uint32_t stream = uint32_t(wk) * STAGES * STAGE, buf0 = lds0 + stream;
-    const int32_t k_first = kb + wk * KW;
     if (k_first < ke) {
         issue(k_first, kpool, koff, kin, buf0);
         issue(k_first, vpool, voff, vin, buf0 + KB);
@@ -599,15 +695,22 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         if (seen) {
             const bool full = lo_all <= kt && hi_all >= kt + KW;
             if (capped || biased || sc == 0.f) {  // (a scale of zero times a masked score is no number)
+                const float from = float(pos - kt - 4 * lh);  // this row's distance to the lane's first key
 #pragma unroll
                 for (int j = 0; j < NSUB; ++j)
 #pragma unroll
                     for (int i = 0; i < AV; ++i) {
                         float z = s[j][i] * sc;
-                        if (capped) z = cap2 * tanh_f<kSplit>(z);
-                        if (biased) z -= slope * fabsf(float(pos - kt - key_in(j, i)));
+                        if (capped) z = tanh_f<kSplit>(z, cap2);
                         s[j][i] = z;
                     }
+                if (biased) {
+#pragma unroll
+                    for (int j = 0; j < NSUB; ++j)
+#pragma unroll
+                        for (int i = 0; i < AV; ++i)
+                            s[j][i] = fmaf(-slope, fabsf(from - float(SUB * j + (NQ == 32 ? (i & 3) + 8 * (i >> 2) : i))), s[j][i]);
+                }
                 unit = 1.f;
             }
             if (!full) {
@@ -681,24 +784,29 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     l = rows_sum<NQ>(l);
 
     T *out = static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * hd;
-    const int64_t part = (int64_t(row) * a.heads + head) * a.slots + (GROUPS ? 0 : a.gsplits) + split;
-    if constexpr (WK == 1) {
-        if (!valid) return;
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-        if (!whole && lh == 0) {
-            a.ml[2 * part] = m;
-            a.ml[2 * part + 1] = l;
+    const int64_t rh = int64_t(row) * a.heads + head, part = rh * a.slots + (GROUPS ? 0 : a.gsplits) + split;
+    auto put = [&](int e, f32x4 x, float inv) {
+        if (whole) {
+            store4(out + e, x * inv);
+        } else if (a.count) {
+            put_far(a.po + part * hd + e, x[0], x[1]);
+            put_far(a.po + part * hd + e + 2, x[2], x[3]);
+        } else {
+            *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
         }
+    };
+    if constexpr (WK == 1) {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        if (valid) {
+            if (!whole && lh == 0) put_far(a.ml + 2 * part, m, l);
 #pragma unroll
-        for (int d = 0; d < ND; ++d)
+            for (int d = 0; d < ND; ++d)
 #pragma unroll
-            for (int i = 0; i < AV; i += 4) {
-                const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
-                if (e >= hd) continue;
-                const f32x4 x = {o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
-                if (whole) store4(out + e, x * inv);
-                else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
-            }
+                for (int i = 0; i < AV; i += 4) {
+                    const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
+                    if (e < hd) put(e, f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]}, inv);
+                }
+        }
     } else {
         // the waves' parts side by side in LDS, then every lane adds its 4 dims of a row, in wave order
         constexpr int LDO = HDP + 4;
@@ -716,9 +824,7 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
                 const int e = NQ * d + (NQ == 32 ? 2 * i + 4 * lh : 4 * lh);
                 *reinterpret_cast<f32x4 *>(so + (wk * NQ + col) * LDO + e) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
             }
-        wait_step<0>();
-        block_barrier();
-        if (!valid) return;
+        read_barrier();
         float M = -INFINITY, L = 0.f, f[WK];
 #pragma unroll
         for (int w = 0; w < WK; ++w) M = fmaxf(M, f[w] = sm[w * NQ + col]);
@@ -728,19 +834,37 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
             L += f[w] * sm[(WK + w) * NQ + col];
         }
         const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-        if (!whole && wave == 0 && lh == 0) {
-            a.ml[2 * part] = M;
-            a.ml[2 * part + 1] = L;
-        }
-        // lane (col, lh) of wave w takes 4 dims at 4 (w (64 / NQ) + lh), and every 4 x 256 / NQ on
-        for (int e = 4 * (wave * (64 / NQ) + lh); e < hd; e += 4 * 256 / NQ) {
-            f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (valid) {
+            if (!whole && wave == 0 && lh == 0) put_far(a.ml + 2 * part, M, L);
+            // lane (col, lh) of wave w takes 4 dims at 4 (w (64 / NQ) + lh), and every 4 x 256 / NQ on
+            for (int e = 4 * (wave * (64 / NQ) + lh); e < hd; e += 4 * 256 / NQ) {
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < WK; ++w) x += *reinterpret_cast<const f32x4 *>(so + (w * NQ + col) * LDO + e) * f[w];
-            if (whole) store4(out + e, x * inv);
-            else *reinterpret_cast<f32x4 *>(a.po + part * hd + e) = x;
+                for (int w = 0; w < WK; ++w) x += *reinterpret_cast<const f32x4 *>(so + (w * NQ + col) * LDO + e) * f[w];
+                put(e, x, inv);
+            }
         }
     }
+    if (whole || !a.count) return;
+    // The last of a row's blocks to come here joins its parts, in slot order whoever it is: they were written past the caches
+    // that other XCDs do not see, before the count (the wait). It leaves the count at zero for the next launch.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    read_barrier();
+    int32_t *mine = reinterpret_cast<int32_t *>(smem);  // of each query row: parts of the group | own << 16 where it is to join, else 0
+    int64_t *which = reinterpret_cast<int64_t *>(smem + 512);
+    if (wk == 0 && lh == 0) {
+        bool last = false;
+        if (valid) {
+            last = __hip_atomic_fetch_add(a.count + rh, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+            if (last) __hip_atomic_store(a.count + rh, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        mine[wq * NQ + col] = last ? gruns | (parts - gruns) << 16 : 0;
+        which[wq * NQ + col] = rh;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    read_barrier();
+    for (int i = int(threadIdx.x) / 32; i < TILE; i += 8)
+        if (mine[i]) join_row<T, true>(a, which[i], mine[i] & 0xFFFF, mine[i] >> 16);
 }
 
 // The tiles of the groups' shared keys (GN query rows a wave, GW waves beside each other; 0: no groups), then those of the
@@ -760,55 +884,14 @@ __global__ __launch_bounds__(256, 2) void k_paged_attn(PagedAttnArgs a) {
     attn_tile<T, C, HDP, SN, SW, false>(a, id, smem);
 }
 
-// The parts of rows whose keys went in several runs, or partly with a group: M = their largest maximum, sums and outputs scaled
-// by 2^(max - M) and added in slot order. desc[row] (0: written already) is the number of a group's parts and, 16 bits up, of
-// the sequence's own. grid x = rows x ceil(heads / 8), block 256: 32 lanes a head, 4 dims each. One round trip finds
-// desc and every slot's maximum and sum (one slot a lane, as many as there are), the next the outputs.
+// The join as a launch of its own, where a block has so many rows that joining them in turn would take longer. desc[row] (0:
+// written already): parts of the group, own parts 16 bits up. grid x = rows x ceil(heads / 8), block 256.
 template <class T>
 __global__ __launch_bounds__(256) void k_paged_join(PagedAttnArgs a) {
     const int hb = (a.heads + 7) / 8, row = int(blockIdx.x) / hb, head = int(blockIdx.x) % hb * 8 + int(threadIdx.x) / 32;
-    const int lane = threadIdx.x & 63, l32 = lane & 31, e = 4 * l32;
-    const bool on = head < a.heads;
-    const int64_t base = (int64_t(row) * a.heads + (on ? head : 0)) * a.slots;
     const int32_t r0 = a.b.row_start[0], r1 = a.b.row_start[a.b.seqs], desc = a.desc[row];
-    float mi[2], li[2];  // slots l32 and 32 + l32
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int64_t at = base + min(32 * k + l32, a.slots - 1);
-        mi[k] = a.ml[2 * at];
-        li[k] = a.ml[2 * at + 1];
-    }
-    if (row < r0 || row >= r1 || desc == 0) return;
-    const int gn = min(desc & 0xFFFF, a.gsplits), sn = min(desc >> 16, a.ssplits);
-    auto used = [&](int i) { return i < gn || (i >= a.gsplits && i < a.gsplits + sn); };
-    float M = -INFINITY, w[2], L = 0.f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        mi[k] = used(32 * k + l32) ? mi[k] : -INFINITY;
-        M = fmaxf(M, mi[k]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        w[k] = mi[k] == -INFINITY ? 0.f : exp2_fast(mi[k] - M);
-        L += used(32 * k + l32) ? w[k] * li[k] : 0.f;  // (a slot that no block wrote holds anything)
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor(L, o, 64);
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    const float *po = a.po + base * a.c.hd + (e < a.c.hd ? e : 0);
-    auto add = [&](int i) {
-        const float f = __shfl(w[i >> 5], (lane & 32) + (i & 31), 64);
-        x += *reinterpret_cast<const f32x4 *>(po + int64_t(i) * a.c.hd) * f;
-    };
-#pragma unroll 4
-    for (int i = 0; i < gn; ++i) add(i);
-#pragma unroll 4
-    for (int i = 0; i < sn; ++i) add(a.gsplits + i);
-    if (!on || e >= a.c.hd) return;
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    store4(static_cast<T *>(a.out) + int64_t(row) * a.ld_out + int64_t(head) * a.c.hd + e, x * inv);
+    if (row < r0 || row >= r1 || desc == 0 || head >= a.heads) return;
+    join_row<T, false>(a, int64_t(row) * a.heads + head, min(desc & 0xFFFF, a.gsplits), min(desc >> 16, a.ssplits));
 }
 
 }  // namespace vh

@@ -339,9 +339,11 @@ struct PagedAttnArgs {
     float scale, cap;
     int32_t *status;
     // the launch (PagedPlan), and the parts of rows whose keys go in several runs: slots of a (row, head), a group's gsplits then a
-    // sequence's ssplits; ml (max, sum) and po [head_dim] of each, desc of each row, behind each other in one workspace
+    // sequence's ssplits; ml (max, sum) and po [head_dim] of each, desc of each row, behind each other in one workspace. count
+    // [rows][heads]: the parts there are, zero between launches (null: k_paged_join joins). magic: 2^32 / (heads / kv_heads) + 1
     float *ml, *po;
-    int32_t *desc;
+    int32_t *count, *desc;
+    uint32_t magic;
     int32_t slots, gsplits, ssplits, gleast, sleast, gtiles, stiles, direct;
 };
 // Where the attention's launches come from: tiles and splits by the batch's bounds, and the floats of its workspace.
@@ -350,7 +352,7 @@ struct PagedPlan {
     int32_t stiles, gtiles;  // at most so many tiles
     int32_t direct;          // tile i is sequence i
     int32_t gsplits, ssplits, gleast, sleast, slots;
-    int64_t ws_floats;
+    int64_t parts, ws_floats, counts;  // counts 0: k_paged_join joins
 };
 
 }  // namespace vh

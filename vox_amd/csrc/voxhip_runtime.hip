@@ -215,9 +215,11 @@ struct Ctx {
     // the range-status word (allocated and zeroed at init) and its pinned host copy; word 1 of the device block is
     // the scratch of the weight max |w| reduction
     int32_t *status_dev = nullptr, *status_pin = nullptr;
-    // parts of the paged-cache attention (paged_ws)
+    // parts of the paged-cache attention and how many of a row there are (paged_ws)
     float *paged_ws = nullptr;
     int64_t paged_ws_floats = 0;
+    int32_t *paged_count = nullptr;
+    int64_t paged_counts = 0;
     // VOXHIP_CHECK_HOST=1 at a voxhip_init call: copy_h2d / copy_d2h check each side's memory type (check_copy_side)
     bool check_copies = false;
 };
@@ -351,6 +353,10 @@ void sync_status() {
     if (v & vh::kStatusFixRange)
         what += std::string(what.empty() ? "" : "; ") + "a fused-FFN term that is not finite or beyond +-2^18 (fixed-point range)";
     std::string where;  // of the paged cache
+    if ((v & vh::kStatusBadBatch) && g.paged_count) {  // a row whose blocks disagree on its parts leaves its count anywhere
+        HIPCHECK(hipMemsetAsync(g.paged_count, 0, size_t(g.paged_counts) * 4, g.stream));
+        HIPCHECK(hipStreamSynchronize(g.stream));
+    }
     if (v & vh::kStatusBadPage) where = "a page table entry outside the pool";
     if (v & vh::kStatusBadBatch)
         where += std::string(where.empty() ? "" : "; ") + "row_start, len or a position outside the batch, its page table or the rope table";
@@ -3985,17 +3991,25 @@ void need_rows(const void *p, int64_t ld, int64_t cols, int32_t type, const char
     if (ld % 8) paged_fail(std::string(what) + ": the row stride is not a multiple of 8");
 }
 
-// The attention's parts, grown when a batch needs more (work in flight on the stream uses the old block until it is waited for).
-float *paged_ws(int64_t floats) {
-    if (g.paged_ws_floats < floats) {
-        HIPCHECK(hipStreamSynchronize(g.stream));
+// The attention's parts and counts, grown when a batch needs more. The counts start at zero and every launch leaves them so.
+void paged_ws(const PagedPlan &p) {
+    if (g.paged_ws_floats < p.ws_floats) {
+        HIPCHECK(hipStreamSynchronize(g.stream));  // work in flight uses the old block
         dfree(g.paged_ws);
         g.paged_ws = nullptr;
         g.paged_ws_floats = 0;
-        g.paged_ws = dalloc_t<float>(size_t(floats));
-        g.paged_ws_floats = floats;
+        g.paged_ws = dalloc_t<float>(size_t(p.ws_floats));
+        g.paged_ws_floats = p.ws_floats;
     }
-    return g.paged_ws;
+    if (g.paged_counts < p.counts) {
+        HIPCHECK(hipStreamSynchronize(g.stream));
+        dfree(g.paged_count);
+        g.paged_count = nullptr;
+        g.paged_counts = 0;
+        g.paged_count = dalloc_t<int32_t>(size_t(p.counts));
+        HIPCHECK(hipMemset(g.paged_count, 0, size_t(p.counts) * 4));
+        g.paged_counts = p.counts;
+    }
 }
 
 int kv_append(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r) {
@@ -4040,6 +4054,7 @@ int attn_paged(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const vox
     need_row_type(r->type, kv->type);
     need(r->heads > 0 && r->heads <= kPagedMaxHeads, "heads out of range");
     need(r->heads % kv->kv_heads == 0, "heads is not a multiple of kv_heads");
+    need(!b || int64_t(b->rows) * r->heads <= (int64_t(1) << 30), "rows x heads out of range");
     need(std::isfinite(r->scale), "scale is not finite");
     need(std::isfinite(r->cap) && r->cap >= 0.f, "cap is negative or not finite");
     need(r->window >= 0, "window is negative");
@@ -4070,7 +4085,8 @@ int attn_paged(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const vox
     const OnDevice on;
     vh::prof_stage("paged");
     const PagedPlan plan = plan_paged_attn(a, b->max_rows, b->max_len, p ? p->max_len : 0);
-    HIPCHECK(launch_paged_attn(r->type, a, plan, paged_ws(plan.ws_floats), g.stream));
+    paged_ws(plan);
+    HIPCHECK(launch_paged_attn(r->type, a, plan, g.paged_ws, g.paged_count, g.stream));
     return 1;
 }
 }  // namespace
