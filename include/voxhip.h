@@ -513,6 +513,28 @@ typedef struct voxhip_shared_prefix {
 int voxhip_attn_shared_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_shared_prefix *p,
                            const voxhip_attn_rows *r);
 
+/* A transformer over a pool: one server's sessions in one call. voxhip_pool_create allocates `pages` pages of page_size positions
+ * (a power of two, 8..1024) for every layer of a transformer (f16, zeros; head sizes that are multiples of 8); a handle or -1.
+ * voxhip_pool_free gives them back. Which session holds which pages is the caller's to keep. */
+int voxhip_pool_create(int xfmr, int32_t pages, int32_t page_size);
+int voxhip_pool_free(int pool);
+/* Host description of a step: rows[s] new rows of sequence s (0: none), len[s] its keys with them (at most 65536), pages
+ * [seqs][page_ld] its table. Groups (0: none) of sequences seq_start[g] .. seq_start[g + 1] - 1 begin with the same shared[g]
+ * keys, in the pages of the group's first sequence. */
+typedef struct voxhip_pool_batch {
+    int32_t seqs;
+    const int32_t *rows, *len, *pages;
+    int64_t page_ld;
+    int32_t groups;
+    const int32_t *seq_start, *shared;
+} voxhip_pool_batch;
+/* All layers over the rows x [sum of rows][hidden] (host; sequence by sequence), their keys and values into the pages, queries
+ * over the pages with voxhip_kv_append_dev's and voxhip_attn_shared_dev's kernels: prompts and steps mixed. out [seqs][hidden] (or NULL) =
+ * final RMSNorm of every sequence's last row; head >= 0: head_out [seqs][head.rows] = head applied to it; sequences without
+ * rows are left as they are in both. The rows' total picks the arithmetic, as m does in voxhip_xfmr_forward. Two sequences that
+ * would write one page, entries outside the pool and rows among shared keys are refused before anything runs. Returns 1 or 0. */
+int voxhip_xfmr_forward_paged(int xfmr, int pool, const voxhip_pool_batch *b, const float *x, float *out, int head, float *head_out);
+
 /* ---------------------------------------------------------------- measurement */
 /* Kernel classes of one decode step, for voxhip_bench_result. */
 enum voxhip_kernel_class {

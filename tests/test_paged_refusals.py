@@ -90,6 +90,33 @@ def test_shared(change, why):
     assert why in error("voxhip_attn_shared_dev", kv, b, sh, at)
 
 
+def pool_step(rows, lens, pages, groups=(), change=()):
+    import numpy as np
+    r, n, p = (np.array(v, np.int32) for v in (rows, lens, pages))
+    starts = np.array([a for a, _, _ in groups] + [groups[-1][1]] if groups else [0], np.int32)
+    shared = np.array([k for _, _, k in groups] or [0], np.int32)
+    b = vh.PoolBatch(len(rows), r.ctypes.data, n.ctypes.data, p.ctypes.data, p.shape[1], len(groups), starts.ctypes.data, shared.ctypes.data)
+    for k, v in change:
+        setattr(b, k, v)
+    x = np.zeros((8, 8), np.float32)
+    assert vh.lib().voxhip_xfmr_forward_paged(0, 0, C.byref(b), x.ctypes.data, None, -1, None) == 0
+    return vh.lib().voxhip_last_error().decode()
+
+
+def test_pool():
+    L = vh.lib()
+    for pages, size in ((0, 16), (-1, 16), (1 << 28, 16)):
+        assert L.voxhip_pool_create(0, pages, size) == -1 and b"pages out of range" in L.voxhip_last_error()
+    for size in (0, 4, 24, 2048):
+        assert L.voxhip_pool_create(0, 4, size) == -1 and b"page_size" in L.voxhip_last_error()
+    assert L.voxhip_pool_free(0) == 0
+    assert "missing" in pool_step([1], [1], [[0]], change=[("rows", None)])
+    assert "missing" in pool_step([1], [1], [[0]], change=[("pages", None)])
+    assert "missing" in pool_step([1], [1], [[0]], change=[("page_ld", 0)])
+    assert L.voxhip_xfmr_forward_paged(0, 0, None, None, None, -1, None) == 0
+    assert L.voxhip_xfmr_forward_paged(0, 0, C.byref(vh.PoolBatch(0)), None, None, -1, None) == 1  # nothing to do
+
+
 def test_missing_structs():
     kv, b, ap, at, sh = parts()
     assert "no cache" in error("voxhip_kv_append_dev", None, b, ap)

@@ -190,6 +190,9 @@ hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s);
 PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_len, int32_t max_shared);
 hipError_t launch_paged_attn(int type, PagedAttnArgs a, const PagedPlan &plan, float *ws, int32_t *count, hipStream_t s);
 
+// Rows ids[0..n) (device, inside src) of src [.][cols] (cols % 4 == 0) one behind the other.
+hipError_t launch_gather_rows(const float *src, int64_t cols, const int32_t *ids, int n, float *out, hipStream_t s);
+
 // Shared-memory opt-in above 64 KiB, once per kernel.
 hipError_t ensure_smem(const void *kernel, size_t bytes);
 

@@ -34,6 +34,11 @@ hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     });
 }
 
+hipError_t launch_gather_rows(const float *src, int64_t cols, const int32_t *ids, int n, float *out, hipStream_t s) {
+    if (n <= 0 || cols <= 0 || cols % 4) return hipErrorInvalidValue;
+    return launch(k_gather_rows, dim3(unsigned(n)), dim3(256), 0, s, src, cols, ids, out);
+}
+
 // Tiles of 16, 32 or 128 query rows by the most that a segment can have; runs so that the launch has a few blocks for each of
 // the 256 CUs, of no fewer than kLeastKeys keys.
 PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_len, int32_t max_shared) {

@@ -121,6 +121,13 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     }
 }
 
+// grid n, block 256: row ids[blockIdx.x] of src to row blockIdx.x of out (the last rows of a ragged batch's sequences).
+static __global__ __launch_bounds__(256) void k_gather_rows(const float *src, int64_t cols, const int32_t *ids, float *out) {
+    const float *from = src + int64_t(ids[blockIdx.x]) * cols;
+    float *to = out + int64_t(blockIdx.x) * cols;
+    for (int64_t i = 4 * int64_t(threadIdx.x); i < cols; i += 1024) *reinterpret_cast<f32x4 *>(to + i) = *reinterpret_cast<const f32x4 *>(from + i);
+}
+
 // ------------------------------------------------------------------ attention
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

@@ -169,6 +169,12 @@ struct Seq {
     int layers = 0, kvh = 0, hd = 0;
 };
 
+// Pages of all layers of a transformer shape: k and v [layers][pages][kv_heads][page_size][head_dim] f16.
+struct Pool {
+    int32_t layers = 0, kvh = 0, hd = 0, pages = 0, page_size = 0;
+    _Float16 *k = nullptr, *v = nullptr;
+};
+
 struct Ctx {
     std::mutex mu;
     bool ok = false;
@@ -215,6 +221,10 @@ struct Ctx {
     // the range-status word (allocated and zeroed at init) and its pinned host copy; word 1 of the device block is
     // the scratch of the weight max |w| reduction
     int32_t *status_dev = nullptr, *status_pin = nullptr;
+    std::vector<Pool> pools;
+    // a paged pass's batch on the device (row starts, lengths, tables, groups, gathered rows) and its pinned copy
+    int32_t *paged_meta = nullptr, *paged_meta_host = nullptr;
+    size_t paged_meta_ints = 0;
     // parts of the paged-cache attention and how many of a row there are (paged_ws)
     float *paged_ws = nullptr;
     int64_t paged_ws_floats = 0;
@@ -1043,16 +1053,17 @@ void enqueue_layers(Xfmr &X, int mc, int64_t m_total, int first, int count, hipS
     if (acc_live) probed(pr, VOXHIP_K_FOLD, [&] { HIPCHECK(launch_acc_fold(X.h, X.acc, X.H, s)); });
 }
 
-// Final RMSNorm of rows [r0, r0 + mr) of X.h into X.xnorm, and the head on them when head >= 0.
-void enqueue_final(Xfmr &X, int r0, int mr, int head, hipStream_t s) {
+// Final RMSNorm of rows [r0, r0 + mr) of X.h (or of `from`) into X.xnorm, and the head on them when head >= 0 (m_total: the
+// caller's rows, which pick the head's arithmetic; 0: mr).
+void enqueue_final(Xfmr &X, int r0, int mr, int head, hipStream_t s, const float *from = nullptr, int64_t m_total = 0) {
+    const float *h = from ? from : X.h + size_t(r0) * X.H;
     if (head >= 0) {
         const GpuMat &Hm = mat_at(head);
         if (Hm.cols != X.H) throw Fail("head width differs from the hidden size");
         float *lg = ensure_logits(X, int64_t(mr) * Hm.rows);
-        gemv(Hm, mr, PRO_RMS, EPI_STORE, X.h + size_t(r0) * X.H, X.H, mr, lg, Hm.rows, X.norms + X.final_off, X.eps,
-             X.xnorm, s);
+        gemv(Hm, m_total ? m_total : mr, PRO_RMS, EPI_STORE, h, X.H, mr, lg, Hm.rows, X.norms + X.final_off, X.eps, X.xnorm, s);
     } else {
-        HIPCHECK(launch_rmsnorm_rows(X.h + size_t(r0) * X.H, X.H, X.norms + X.final_off, X.H, X.eps, X.xnorm, X.H, mr, s));
+        HIPCHECK(launch_rmsnorm_rows(h, X.H, X.norms + X.final_off, X.H, X.eps, X.xnorm, X.H, mr, s));
     }
 }
 
@@ -4089,9 +4100,246 @@ int attn_paged(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const vox
     HIPCHECK(launch_paged_attn(r->type, a, plan, g.paged_ws, g.paged_count, g.stream));
     return 1;
 }
+
+// ------------------------------------------------------------------ a transformer over a pool of pages
+Pool &pool_at(int id) {
+    if (id < 0 || size_t(id) >= g.pools.size() || !g.pools[size_t(id)].k) throw Fail("bad pool handle " + std::to_string(id));
+    return g.pools[size_t(id)];
+}
+PagedKv pool_layer(const Pool &P, int layer) {
+    PagedKv c{};
+    const int64_t page = int64_t(P.kvh) * P.page_size * P.hd;
+    c.k = P.k + size_t(layer) * size_t(P.pages) * size_t(page);
+    c.v = P.v + size_t(layer) * size_t(P.pages) * size_t(page);
+    c.page_stride = page; c.head_stride = int64_t(P.page_size) * P.hd; c.pos_stride = P.hd;
+    c.pages = P.pages; c.kv_heads = P.kvh; c.hd = P.hd;
+    while ((1 << c.shift) < P.page_size) ++c.shift;
+    return c;
+}
+
+// The layers of a ragged pass of mc rows in X.h: as enqueue_layers for any head size, with the append and the attention of the
+// paged cache.
+void enqueue_layers_paged(Xfmr &X, const Pool &P, const PagedBatch &b, const PagedGroups &grp, int32_t max_rows, int32_t max_len,
+                          int32_t max_shared, int64_t m_total, hipStream_t s) {
+    const int mc = b.rows, qd = X.heads * X.hd, ld = qd + 2 * X.kvh * X.hd;
+    for (int li = 0; li < X.layers; ++li) {
+        const LayerDev &L = X.L[size_t(li)];
+        const GpuMat &Mqkv = g.mats[size_t(L.qkv)], &Mo = g.mats[size_t(L.o)], &Mgu = g.mats[size_t(L.gu)], &Md = g.mats[size_t(L.down)];
+        gemv(Mqkv, m_total, PRO_RMS, EPI_STORE, X.h, X.H, mc, X.qkv, ld, X.norms + L.ln1, X.eps, nullptr, s, nullptr, X.pre);
+        AppendArgs ap{};
+        ap.c = pool_layer(P, li); ap.b = b;
+        ap.qkv = X.qkv; ap.q = X.q; ap.ld_qkv = ld; ap.ld_q = qd;
+        if (L.qk) { ap.qn = X.norms + L.qn; ap.kn = X.norms + L.kn; }
+        ap.rope = X.rope; ap.rope_len = int32_t(X.rope_rows); ap.rot = X.hd;
+        ap.heads = X.heads; ap.eps = X.eps;
+        HIPCHECK(launch_kv_append(VOXHIP_F32, ap, s));
+        PagedAttnArgs at{};
+        at.c = ap.c; at.b = b; at.p = grp;
+        at.q = X.q; at.out = X.pre; at.ld_q = at.ld_out = qd;
+        at.heads = X.heads; at.scale = 1.0f / std::sqrt(float(X.hd));
+        const PagedPlan plan = plan_paged_attn(at, max_rows, max_len, max_shared);
+        paged_ws(plan);
+        HIPCHECK(launch_paged_attn(VOXHIP_F32, at, plan, g.paged_ws, g.paged_count, s));
+        gemv(Mo, m_total, PRO_X, EPI_ACC, X.pre, qd, mc, X.h, X.H, nullptr, 0.f, nullptr, s);
+        QRows gq{};
+        const bool gq_on = ffn_quant_epilogue(Mgu, Md, m_total, mc, lib_scratch(), &gq);
+        gemv(Mgu, m_total, PRO_RMS, EPI_SWIGLU, X.h, X.H, mc, X.g, X.I, X.norms + L.ln2, X.eps, nullptr, s, nullptr, X.pre, nullptr,
+             nullptr, nullptr, nullptr, gq_on ? &gq : nullptr);
+        gemv(Md, m_total, PRO_X, EPI_ACC, X.g, X.I, mc, X.h, X.H, nullptr, 0.f, nullptr, s, nullptr, nullptr, nullptr, nullptr, nullptr,
+             nullptr, nullptr, gq_on ? &gq : nullptr);
+    }
+}
+
+int forward_paged(int xfmr, int pool, const voxhip_pool_batch *b, const float *x, float *out, int head, float *head_out) {
+    // the batch first: what a caller got wrong never reaches the device
+    need(b && b->seqs >= 0 && b->seqs <= kPagedMaxSeqs, "no batch, or too many sequences");
+    if (b->seqs == 0) return 1;
+    need(b->rows && b->len && b->pages && b->page_ld > 0, "rows, len or pages is missing");
+    need(x, "no input rows");
+    require_ok();
+    Xfmr &X = xf_at(xfmr);
+    const Pool P = pool_at(pool);
+    need(P.layers >= X.layers && P.kvh == X.kvh && P.hd == X.hd, "the pool belongs to another transformer shape");
+    const int S = b->seqs;
+    std::vector<int32_t> shared(size_t(S), 0), lead(size_t(S), -1);
+    const int n_groups = b->groups > 0 && b->seq_start && b->shared ? b->groups : 0;
+    need(b->groups >= 0 && b->groups <= S && (b->groups == 0 || n_groups), "more groups than sequences, or their arrays are missing");
+    int32_t max_shared = 0;
+    for (int q = 0; q < n_groups; ++q) {
+        need(b->seq_start[q] >= 0 && b->seq_start[q] <= b->seq_start[q + 1] && b->seq_start[q + 1] <= S, "a group's sequences are out of order");
+        need(b->shared[q] >= 0, "a group's shared keys are negative");
+        for (int s = b->seq_start[q]; s < b->seq_start[q + 1]; ++s) {
+            shared[size_t(s)] = b->shared[q];
+            lead[size_t(s)] = b->seq_start[q];
+        }
+        max_shared = std::max(max_shared, b->shared[q]);
+    }
+    int64_t total = 0;
+    int32_t max_len = 1, n_out = 0;
+    std::unordered_map<int32_t, int> writer;  // page -> the sequence whose rows it gets
+    for (int s = 0; s < S; ++s) {
+        const int32_t n = b->rows[s], len = b->len[s];
+        need(n >= 0 && len >= n, "rows is negative, or more than len");
+        need(len <= kMaxCap && (int64_t(len) + P.page_size - 1) / P.page_size <= b->page_ld, "len exceeds the page table");
+        need(n == 0 || len - n >= shared[size_t(s)], "a sequence's rows lie among its group's shared keys");
+        if (n && lead[size_t(s)] >= 0) need(shared[size_t(s)] <= b->len[lead[size_t(s)]], "a group shares more keys than its first sequence has");
+        if (n) {
+            const int32_t *own = b->pages + int64_t(s) * b->page_ld, *first = lead[size_t(s)] >= 0 ? b->pages + int64_t(lead[size_t(s)]) * b->page_ld : own;
+            for (int32_t p = 0; p * P.page_size < len; ++p) {
+                // a page that the shared keys fill is the first sequence's; one that they end in is both's
+                if (p * P.page_size < shared[size_t(s)]) need(first[p] >= 0 && first[p] < P.pages, "a page table entry outside the pool");
+                if ((p + 1) * P.page_size > shared[size_t(s)]) need(own[p] >= 0 && own[p] < P.pages, "a page table entry outside the pool");
+                if ((p + 1) * P.page_size > len - n) {
+                    const auto it = writer.emplace(own[p], s);
+                    need(it.second || it.first->second == s, "two sequences write one page");
+                }
+            }
+            ++n_out;
+        }
+        total += n;
+        max_len = std::max(max_len, len);
+    }
+    need(total <= kPagedMaxRows, "too many rows");
+    if (!total) return 1;
+    ensure_rope(X, max_len);
+    const int64_t H = X.H;
+    int chunk = kMaxPass;
+    for (const LayerDev &L : X.L)
+        for (int id : {L.qkv, L.o, L.gu, L.down}) chunk = std::min(chunk, rows_per_pass(g.mats[size_t(id)], total));
+    const int64_t V = head >= 0 ? mat_at(head).rows : 0;
+    if (head >= 0) chunk = std::min(chunk, rows_per_pass(mat_at(head), n_out));
+    chunk = int(std::min<int64_t>(chunk, total));
+    ensure_rows(X, chunk);
+    const OnDevice on;
+    vh::prof_stage(X.name.c_str());
+    const size_t ints = size_t(S) * (2 + size_t(b->page_ld)) + 1 + 2 * size_t(n_groups) + 1 + size_t(chunk);
+    if (g.paged_meta_ints < ints) {
+        HIPCHECK(hipStreamSynchronize(g.stream));
+        dfree(g.paged_meta);
+        if (g.paged_meta_host) (void)hipHostFree(g.paged_meta_host);
+        g.paged_meta = g.paged_meta_host = nullptr;
+        g.paged_meta_ints = 0;
+        g.paged_meta = dalloc_t<int32_t>(ints);
+        HIPCHECK(hipHostMalloc(reinterpret_cast<void **>(&g.paged_meta_host), ints * 4, hipHostMallocDefault));
+        g.paged_meta_ints = ints;
+    }
+    float *pin = pinned(size_t(chunk) * size_t(std::max(H, V)) * 4 + 64);
+    int64_t at = 0;       // rows done
+    int seq = 0, in = 0;  // the next row's sequence and index in it
+    for (; at < total;) {
+        const int mc = int(std::min<int64_t>(chunk, total - at));
+        HIPCHECK(hipStreamSynchronize(g.stream));  // the pinned blocks may still feed an earlier copy
+        // this pass: the rows of sequences seq .. as far as mc goes; the others have none
+        int32_t *start = g.paged_meta_host, *len = start + S + 1, *table = len + S, *gs = table + size_t(S) * size_t(b->page_ld),
+                *gl = gs + n_groups + 1, *pick = gl + n_groups;
+        std::memcpy(table, b->pages, size_t(S) * size_t(b->page_ld) * 4);
+        if (n_groups) {
+            std::memcpy(gs, b->seq_start, size_t(n_groups + 1) * 4);
+            std::memcpy(gl, b->shared, size_t(n_groups) * 4);
+        }
+        std::vector<int> ends;  // sequences whose last row is in this pass
+        int32_t max_rows = 1;
+        start[0] = 0;
+        int left = mc, s0 = seq, i0 = in;
+        for (int s = 0; s < S; ++s) {
+            const int before = s == s0 ? i0 : 0;
+            int n = s < s0 ? 0 : std::min(left, b->rows[s] - before);
+            start[s + 1] = start[s] + n;
+            len[s] = b->len[s] - b->rows[s] + (s < s0 ? b->rows[s] : before + n);
+            left -= n;
+            max_rows = std::max(max_rows, n);
+            if (n && before + n == b->rows[s]) {
+                pick[ends.size()] = start[s + 1] - 1;
+                ends.push_back(s);
+            }
+            if (s >= s0 && n) {
+                seq = s;
+                in = before + n;
+            }
+        }
+        if (in == b->rows[seq]) {
+            ++seq;
+            in = 0;
+        }
+        HIPCHECK(copy_h2d(g.paged_meta, g.paged_meta_host, ints * 4, g.stream));
+        std::memcpy(pin, x + at * H, size_t(mc) * size_t(H) * 4);
+        HIPCHECK(copy_h2d(X.h, pin, size_t(mc) * size_t(H) * 4, g.stream));
+        PagedBatch pb{};
+        pb.row_start = g.paged_meta; pb.len = pb.row_start + S + 1; pb.table = pb.len + S;
+        pb.page_ld = b->page_ld; pb.seqs = S; pb.rows = mc;
+        PagedGroups pg{};
+        if (n_groups) {
+            pg.seq_start = pb.table + size_t(S) * size_t(b->page_ld); pg.len = pg.seq_start + n_groups + 1;
+            pg.groups = n_groups;
+        }
+        for (const LayerDev &L : X.L)
+            for (int id : {L.qkv, L.o, L.gu, L.down}) prepare_mat(g.mats[size_t(id)], total, mc, g.stream);
+        enqueue_layers_paged(X, P, pb, pg, max_rows, max_len, max_shared, total, g.stream);
+        const int mr = int(ends.size());
+        if (mr && (out || head >= 0)) {
+            if (head >= 0) prepare_mat(mat_at(head), n_out, mr, g.stream);
+            HIPCHECK(launch_gather_rows(X.h, H, g.paged_meta + (pick - g.paged_meta_host), mr, X.pre, g.stream));
+            enqueue_final(X, 0, mr, head, g.stream, X.pre, n_out);
+            auto give = [&](const float *dev, int64_t w, float *to) {
+                HIPCHECK(copy_d2h(pin, dev, size_t(mr) * size_t(w) * 4, g.stream));
+                HIPCHECK(hipStreamSynchronize(g.stream));
+                for (int i = 0; i < mr; ++i) std::memcpy(to + int64_t(ends[size_t(i)]) * w, pin + int64_t(i) * w, size_t(w) * 4);
+            };
+            if (out) give(X.xnorm, H, out);
+            if (head >= 0 && head_out) give(X.logits, V, head_out);
+        }
+        at += mc;
+    }
+    sync_status();
+    return 1;
+}
 }  // namespace
 
 extern "C" {
+int voxhip_pool_create(int xfmr, int32_t pages, int32_t page_size) {
+    return guard_int([&] {
+        need(page_size >= 8 && page_size <= 1024 && (page_size & (page_size - 1)) == 0, "page_size is a power of two from 8 to 1024");
+        need(pages > 0 && int64_t(pages) * page_size <= kPagedMaxKeys, "pages out of range");
+        require_ok();
+        const Xfmr &X = xf_at(xfmr);
+        need(X.hd % 8 == 0, "the paged cache takes head sizes that are multiples of 8");
+        const OnDevice on;
+        Pool P;
+        P.layers = X.layers; P.kvh = X.kvh; P.hd = X.hd; P.pages = pages; P.page_size = page_size;
+        const size_t n = size_t(X.layers) * size_t(pages) * size_t(X.kvh) * size_t(page_size) * size_t(X.hd);
+        P.k = dalloc_t<_Float16>(n);
+        try {
+            P.v = dalloc_t<_Float16>(n);
+            HIPCHECK(hipMemset(P.k, 0, n * 2));
+            HIPCHECK(hipMemset(P.v, 0, n * 2));
+        } catch (...) {
+            dfree(P.k);
+            dfree(P.v);
+            throw;
+        }
+        for (size_t i = 0; i < g.pools.size(); ++i)
+            if (!g.pools[i].k) {
+                g.pools[i] = P;
+                return int(i);
+            }
+        g.pools.push_back(P);
+        return int(g.pools.size()) - 1;
+    }, -1);
+}
+int voxhip_pool_free(int pool) {
+    return guard_int([&] {
+        require_ok();
+        Pool &P = pool_at(pool);
+        HIPCHECK(hipStreamSynchronize(g.stream));
+        dfree(P.k);
+        dfree(P.v);
+        P = Pool{};
+        return 1;
+    }, 0);
+}
+int voxhip_xfmr_forward_paged(int xfmr, int pool, const voxhip_pool_batch *b, const float *x, float *out, int head, float *head_out) {
+    return guard_int([&] { return forward_paged(xfmr, pool, b, x, out, head, head_out); }, 0);
+}
 int voxhip_kv_append_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b, const voxhip_append_rows *r) {
     return guard_int([&] { return kv_append(kv, b, r); }, 0);
 }

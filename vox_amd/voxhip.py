@@ -164,6 +164,11 @@ class SharedPrefix(C.Structure):
     _fields_ = [("groups", C.c_int32), ("max_len", C.c_int32), ("seq_start", C.c_void_p), ("len", C.c_void_p)]
 
 
+class PoolBatch(C.Structure):
+    _fields_ = [("seqs", C.c_int32), ("rows", C.c_void_p), ("len", C.c_void_p), ("pages", C.c_void_p), ("page_ld", C.c_int64),
+                ("groups", C.c_int32), ("seq_start", C.c_void_p), ("shared", C.c_void_p)]
+
+
 KERNEL_CLASSES = ("qkv_gemv", "o_gemv", "gateup_gemv", "down_gemv", "head_gemv", "attention", "attn_combine", "qk_post", "sampler",
                   "ffn", "acc_fold", "quant_rows")
 
@@ -245,6 +250,9 @@ SIGNATURES = {
     "voxhip_kv_append_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(AppendRows)]),
     "voxhip_attn_paged_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(AttnRows)]),
     "voxhip_attn_shared_dev": (_I, [C.POINTER(PagedKv), C.POINTER(PagedBatch), C.POINTER(SharedPrefix), C.POINTER(AttnRows)]),
+    "voxhip_pool_create": (_I, [_I, _I32, _I32]),
+    "voxhip_pool_free": (_I, [_I]),
+    "voxhip_xfmr_forward_paged": (_I, [_I, _I, C.POINTER(PoolBatch), _P, _P, _I, _P]),
     "voxhip_bench_decode": (_I, [_I, _I, _I64, _P, _I, C.POINTER(SampleCfg), _P, _I, _I, C.POINTER(BenchResult)]),
     "voxhip_bench_decode_steps": (_I, [_I, _P, _P, _I64, _P, _I, _P, _P, _I, _I, C.POINTER(BenchResult)]),
     "voxhip_bench_gemv_q8": (_I, [_I64, _I64, _I, _I, _I, C.POINTER(C.c_double)]),
@@ -904,6 +912,32 @@ def attn_paged_dev(kv, batch, rows):
 def attn_shared_dev(kv, batch, shared, rows):
     """attn_paged_dev with the shared keys of groups of sequences read once for all of a group's rows."""
     _check(lib().voxhip_attn_shared_dev(C.byref(kv), C.byref(batch), C.byref(shared), C.byref(rows)), "attn_shared_dev")
+
+
+def pool_create(xfmr, pages, page_size):
+    return _handle(lib().voxhip_pool_create(xfmr, pages, page_size), "pool_create")
+
+
+def pool_free(pool):
+    _check(lib().voxhip_pool_free(pool), "pool_free")
+
+
+def forward_paged(xfmr, pool, rows, lens, pages, x, hidden, head=-1, groups=()):
+    """One step of a server's sessions: rows / lens [seqs], pages [seqs][page_ld] (host), x [sum(rows)][hidden]. groups: (first
+    sequence, one behind the last, shared keys), in order and side by side. Returns (out [seqs][hidden], head_out or None);
+    sequences without rows get zeros."""
+    x = f32(x)
+    r, n = np.ascontiguousarray(rows, np.int32), np.ascontiguousarray(lens, np.int32)
+    p = np.ascontiguousarray(pages, np.int32).reshape(r.size, -1)
+    starts = np.array([a for a, _, _ in groups] + [groups[-1][1]] if groups else [0], np.int32)
+    shared = np.array([k for _, _, k in groups] or [0], np.int32)
+    if any(a[1] != b[0] for a, b in zip(groups, groups[1:])):
+        raise VoxHipError("forward_paged: groups are not side by side (a group of no shared keys fills a gap)")
+    b = PoolBatch(r.size, r.ctypes.data, n.ctypes.data, p.ctypes.data, p.shape[1], len(groups), starts.ctypes.data, shared.ctypes.data)
+    out = np.zeros((r.size, hidden), np.float32)
+    head_out = np.zeros((r.size, mat_shape(head)[0]), np.float32) if head >= 0 else None
+    _check(lib().voxhip_xfmr_forward_paged(xfmr, pool, C.byref(b), _p(x), _p(out), head, _p(head_out)), "xfmr_forward_paged")
+    return out, head_out
 
 
 def bench_decode(xfmr, seq, pos0, d_x, head, cfg, d_token, warmup, steps):
