@@ -39,27 +39,30 @@ hipError_t launch_gather_rows(const float *src, int64_t cols, const int32_t *ids
     return launch(k_gather_rows, dim3(unsigned(n)), dim3(256), 0, s, src, cols, ids, out);
 }
 
-// Tiles of 16, 32 or 128 query rows by the most that a segment can have; runs so that the launch has a few blocks for each of
-// the 256 CUs, of no fewer than kLeastKeys keys.
+// Tiles of 16, 32 or 128 query rows by the most that a segment can have; runs so that the launch has two blocks for each of the
+// 256 CUs. A run is at least what the four waves of a small tile read at once (128 keys; 256 instead: a session's step behind
+// 512 keys 11.7 instead of 10.4 us, eight behind 1024 15.1 instead of 14.1), of a group's tall tile 256 keys in at most 16 runs
+// (64 rows behind 8192 keys: 44 us, in 32 runs 49, whose parts have to be written and read again).
 PagedPlan plan_paged_attn(const PagedAttnArgs &a, int32_t max_rows, int32_t max_len, int32_t max_shared) {
-    constexpr int32_t kLeastKeys = 256, kMostSplits = 32, kBlocks = 512;
+    constexpr int32_t kBlocks = 512;
     const int32_t G = a.c.kv_heads, group = a.heads / G;
     auto tile_for = [](int64_t q) { return q <= 16 ? 16 : q <= 32 ? 32 : 128; };
-    auto splits_for = [&](int64_t tiles, int32_t keys) {
-        const int64_t want = (kBlocks + tiles * G - 1) / (tiles * G), most = (int64_t(keys) + kLeastKeys - 1) / kLeastKeys;
-        return int32_t(std::max<int64_t>(1, std::min<int64_t>({want, most, kMostSplits})));
+    auto splits_for = [&](int64_t tiles, int32_t keys, int32_t least, int32_t limit) {
+        const int64_t want = (kBlocks + tiles * G - 1) / (tiles * G), most = (int64_t(keys) + least - 1) / least;
+        return int32_t(std::max<int64_t>(1, std::min<int64_t>({want, most, limit})));
     };
     PagedPlan p{};
-    p.gleast = p.sleast = kLeastKeys;
+    p.sleast = 128;
     const int64_t q = int64_t(a.b.rows) * group;
     p.stile = tile_for(int64_t(max_rows) * group);
     p.direct = int64_t(max_rows) * group <= p.stile;
     p.stiles = int32_t(p.direct ? a.b.seqs : std::min<int64_t>(q / p.stile + a.b.seqs, INT32_MAX));
-    p.ssplits = splits_for(p.stiles, max_len);
+    p.ssplits = splits_for(p.stiles, max_len, p.sleast, p.stile == 128 ? 16 : 32);
     if (a.p.groups) {
         p.gtile = tile_for(q);
         p.gtiles = int32_t(q / p.gtile + a.p.groups);
-        p.gsplits = splits_for(std::max<int64_t>(1, q / p.gtile), std::max(max_shared, 1));
+        p.gleast = p.gtile == 128 ? 256 : 128;
+        p.gsplits = splits_for(std::max<int64_t>(1, q / p.gtile), std::max(max_shared, 1), p.gleast, p.gtile == 128 ? 16 : 32);
     }
     p.slots = p.gsplits + p.ssplits;
     if (p.gsplits || p.ssplits > 1) {
