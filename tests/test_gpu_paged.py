@@ -91,7 +91,7 @@ def turned(x, w, eps, rope, rot, inter):
 @pytest.mark.parametrize("hd,heads,kv_heads,rot,inter,norm,nhd,page,gap", [
     (64, 14, 2, 64, False, False, False, 16, 0), (128, 16, 8, 128, False, True, False, 64, 0), (128, 4, 4, 64, True, True, True, 8, 24),
     (80, 5, 1, 40, False, True, False, 32, 8), (96, 6, 3, 96, True, False, True, 128, 0), (40, 3, 1, 8, False, True, False, 16, 0),
-    (8, 2, 1, 8, True, True, False, 8, 0), (64, 4, 2, 0, False, True, True, 16, 0)])
+    (8, 2, 1, 8, True, True, False, 8, 0), (64, 4, 2, 0, False, True, True, 16, 0), (48, 2, 1, 24, False, True, False, 16, 0), (72, 3, 1, 72, True, True, False, 16, 0)])
 def test_append(hip, wtype, hd, heads, kv_heads, rot, inter, norm, nhd, page, gap):
     rows, lens = [5, 0, 1, 17, 3, 2], [5, 9, 40, 17, 200, 1]  # the last has a row at position -1
     b = Batch(rows, lens, wtype, heads, kv_heads, hd, page, seed=hd + rot, pad_rows=3, nhd=nhd, gap=gap)

@@ -19,7 +19,9 @@ hipError_t by_type(int type, F &&f) {
 
 hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     if (a.c.hd <= 0 || a.c.hd > 128 || a.c.hd % 8 || a.b.rows <= 0 || a.b.seqs <= 0) return hipErrorInvalidValue;
-    const int lph = a.c.hd <= 64 ? 16 : 32, per = 256 / lph;
+    // 8 values a lane (16 bytes of a 16-bit row) where a lane's pairs are one lane's too
+    const bool wide = type != WT_F32 && (!a.rope || a.interleaved || a.rot % 16 == 0);
+    const int lph = (a.c.hd <= 64 ? 16 : 32) / (wide ? 2 : 1), per = 256 / lph;
     // turns of heads per row as blocks of their own up to about 2048 blocks (8 a CU), which hide each other's chains of reads
     const int64_t turns = (a.heads + 2 * a.c.kv_heads + per - 1) / per;
     a.blocks = int32_t(std::max<int64_t>(1, std::min<int64_t>(turns, 2048 / a.b.rows)));
@@ -29,8 +31,10 @@ hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     return by_type(type, [&](auto t, auto c) {
         using T = decltype(t);
         using C = decltype(c);
-        return lph == 16 ? launch(k_kv_append<T, C, 16>, dim3(unsigned(grid)), dim3(256), 0, s, a)
-                         : launch(k_kv_append<T, C, 32>, dim3(unsigned(grid)), dim3(256), 0, s, a);
+        const dim3 gr{unsigned(grid)}, bl{256};
+        if constexpr (!std::is_same<T, float>::value)
+            if (wide) return lph == 8 ? launch(k_kv_append<T, C, 8, 8>, gr, bl, 0, s, a) : launch(k_kv_append<T, C, 16, 8>, gr, bl, 0, s, a);
+        return lph == 16 ? launch(k_kv_append<T, C, 16, 4>, gr, bl, 0, s, a) : launch(k_kv_append<T, C, 32, 4>, gr, bl, 0, s, a);
     });
 }
 

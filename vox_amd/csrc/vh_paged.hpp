@@ -26,28 +26,37 @@ VH_DEV int32_t find_seq(const PagedBatch &b, int32_t row) {
     return lo < b.seqs ? lo : -1;
 }
 
-template <class T>
-VH_DEV f32x4 load4(const T *p) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    const t4 v = *reinterpret_cast<const t4 *>(p);
-    return f32x4{float(v[0]), float(v[1]), float(v[2]), float(v[3])};
+template <class T, int N = 4>
+VH_DEV void load_n(const T *p, float (&x)[N]) {
+    typedef T tn __attribute__((ext_vector_type(N)));
+    const tn v = *reinterpret_cast<const tn *>(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = float(v[i]);
+}
+template <class T, int N>
+VH_DEV void store_n(T *p, const float (&x)[N]) {
+    typedef T tn __attribute__((ext_vector_type(N)));
+    tn v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = T(x[i]);
+    *reinterpret_cast<tn *>(p) = v;
 }
 template <class T>
 VH_DEV void store4(T *p, f32x4 v) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
-    *reinterpret_cast<t4 *>(p) = t4{T(v[0]), T(v[1]), T(v[2]), T(v[3])};
+    const float x[4] = {v[0], v[1], v[2], v[3]};
+    store_n(p, x);
 }
 
-// One head of one row per LPH lanes, 4 neighbouring values a lane, 256 / LPH heads at a time; grid x = rows x a.blocks, block 256:
-// block i of a row takes its heads in turns i, i + a.blocks, ... (one each for a step's few rows, all of them where rows
-// alone fill the chip: a block's chain of dependent reads, not the bytes, is what a row costs). A
-// lane of a rotated head also loads the 4 values its own are paired with (halves: rot / 2 away, in L1 by then;
-// interleaved: among its own), so no value crosses lanes but the norm's sum. Rows behind the last sequence, and rows at
-// negative positions, write nothing.
-template <class T, class C, int LPH>
+// One head of one row per LPH lanes, N neighbouring values a lane (16 bytes of a row where halves of the rotation allow it, else 4
+// values), 256 / LPH heads at a time; grid x = rows x a.blocks, block 256: block i of a row takes its heads in turns i, i +
+// a.blocks, ... (one each for a step's few rows, all of them where rows alone fill the chip: a block's chain of dependent
+// reads, not the bytes, is what a row costs). A lane of a rotated head also loads the N values its own are paired with
+// (halves: rot / 2 away, in L1 by then; interleaved: among its own), so no value crosses lanes but the norm's sum. Rows behind
+// the last sequence, and rows at negative positions, write nothing.
+template <class T, class C, int LPH, int N>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     const int row = int(blockIdx.x) / a.blocks;
-    const int e = 4 * (int(threadIdx.x) % LPH);
+    const int e = N * (int(threadIdx.x) % LPH);
     const int hd = a.c.hd, G = a.c.kv_heads, heads = a.heads + 2 * G;
     const int32_t s = find_seq(a.b, row);
     if (s < 0) return;
@@ -62,62 +71,84 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
     const int32_t page = page_of(a.c, a.b.table + int64_t(s) * a.b.page_ld, pos);
     const T *from = static_cast<const T *>(a.qkv) + int64_t(row) * a.ld_qkv;
     const int half = a.rot >> 1, ec = e < hd ? e : 0;
-    const bool inside = a.rope && ec < a.rot;
-    // (cos, sin) of this lane's pairs: four pairs of the halves, or two of neighbours
-    f32x4 cs0 = {1.f, 0.f, 1.f, 0.f}, cs1 = cs0;
+    const bool inside = a.rope && ec < a.rot, low = ec < half;
+    // this lane's cosines and sines: of N pairs of the halves, or of N / 2 of neighbours
+    float cs[N], sn[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        cs[i] = 1.f;
+        sn[i] = 0.f;
+    }
     if (inside) {
-        const float *rp = a.rope + int64_t(pos) * a.rot;
-        if (a.interleaved) {
-            cs0 = *reinterpret_cast<const f32x4 *>(rp + ec);
-        } else {
-            const float *r = rp + 2 * (ec < half ? ec : ec - half);
-            cs0 = *reinterpret_cast<const f32x4 *>(r);
-            cs1 = *reinterpret_cast<const f32x4 *>(r + 4);
+        const float *rp = a.rope + int64_t(pos) * a.rot + (a.interleaved ? ec : 2 * (low ? ec : ec - half));
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            if (a.interleaved) {
+                cs[i] = cs[i + 1] = rp[i];
+                sn[i + 1] = rp[i + 1];
+                sn[i] = -sn[i + 1];
+            } else {
+                cs[i] = rp[2 * i];
+                cs[i + 1] = rp[2 * i + 2];
+                sn[i] = low ? -rp[2 * i + 1] : rp[2 * i + 1];
+                sn[i + 1] = low ? -rp[2 * i + 3] : rp[2 * i + 3];
+            }
         }
     }
-    const int pe = !inside || a.interleaved ? ec : ec < half ? ec + half : ec - half;
+    const int pe = !inside || a.interleaved ? ec : low ? ec + half : ec - half;
     constexpr int PER = 256 / LPH;
     // the first values of the next turn are loaded during this one
     auto head_of = [&](int turn) { return (int(blockIdx.x) % a.blocks + turn * a.blocks) * PER + int(threadIdx.x) / LPH; };
-    auto clamped = [&](int hh) { return hh < heads ? hh : heads - 1; };
+    auto values = [&](int turn, float (&x)[N], float (&xp)[N]) {
+        const T *src = from + int64_t(min(head_of(turn), heads - 1)) * hd;
+        load_n(src + ec, x);
+        load_n(src + pe, xp);
+    };
     const int turns = ((heads + PER - 1) / PER + a.blocks - 1) / a.blocks;
-    f32x4 nx = load4(from + int64_t(clamped(head_of(0))) * hd + ec), np = load4(from + int64_t(clamped(head_of(0))) * hd + pe);
+    float nx[N], np[N];
+    values(0, nx, np);
     for (int k = 0; k < turns; ++k) {
-        const int hh = head_of(k), hc = clamped(hh);
+        const int hh = head_of(k), hc = min(hh, heads - 1);
         const bool on = hh < heads && e < hd, is_q = hc < a.heads, is_v = hc >= a.heads + G;
-        f32x4 x = nx, xp = np;
-        if (k + 1 < turns) {
-            const T *src = from + int64_t(clamped(head_of(k + 1))) * hd;
-            nx = load4(src + ec);
-            np = load4(src + pe);
+        float x[N], xp[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            x[i] = nx[i];
+            xp[i] = np[i];
         }
+        if (k + 1 < turns) values(k + 1, nx, np);
         const float *nw = is_v ? nullptr : is_q ? a.qn : a.kn;
         if (nw) {  // a head's lanes share the branch
-            const f32x4 w = *reinterpret_cast<const f32x4 *>(nw + ec), wp = *reinterpret_cast<const f32x4 *>(nw + pe);
-            const float ss = group_sum<LPH>(e < hd ? x[0] * x[0] + x[1] * x[1] + (x[2] * x[2] + x[3] * x[3]) : 0.f);
+            float w[N], wp[N], ss = 0.f;
+            load_n(nw + ec, w);
+            load_n(nw + pe, wp);
+#pragma unroll
+            for (int i = 0; i < N; ++i) ss = fmaf(x[i], x[i], ss);
+            ss = group_sum<LPH>(e < hd ? ss : 0.f);
             const float inv = 1.0f / sqrtf(ss / float(hd) + a.eps);
-            x = w * (x * inv);
-            xp = wp * (xp * inv);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                x[i] = w[i] * (x[i] * inv);
+                xp[i] = wp[i] * (xp[i] * inv);
+            }
         }
         if (!on) continue;
         if (inside && !is_v) {
-            if (a.interleaved) {
-                x = f32x4{x[0] * cs0[0] - x[1] * cs0[1], x[1] * cs0[0] + x[0] * cs0[1], x[2] * cs0[2] - x[3] * cs0[3],
-                          x[3] * cs0[2] + x[2] * cs0[3]};
-            } else {
-                const f32x4 c = {cs0[0], cs0[2], cs1[0], cs1[2]}, sn = {cs0[1], cs0[3], cs1[1], cs1[3]};
-                x = ec < half ? x * c - xp * sn : x * c + xp * sn;
-            }
+            float y[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] = x[i] * cs[i] + (a.interleaved ? x[i ^ 1] : xp[i]) * sn[i];
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = y[i];
         }
         if (is_q) {
-            if (a.q) store4(static_cast<T *>(a.q) + int64_t(row) * a.ld_q + int64_t(hc) * hd + ec, x);
+            if (a.q) store_n(static_cast<T *>(a.q) + int64_t(row) * a.ld_q + int64_t(hc) * hd + ec, x);
             continue;
         }
         if (page < 0) {
             raise_status(a.status, true, kStatusBadPage);
             continue;
         }
-        store4(static_cast<C *>(is_v ? a.c.v : a.c.k) + key_offset(a.c, page, hc - a.heads - (is_v ? G : 0), pos) + ec, x);
+        store_n(static_cast<C *>(is_v ? a.c.v : a.c.k) + key_offset(a.c, page, hc - a.heads - (is_v ? G : 0), pos) + ec, x);
     }
 }
 
@@ -330,6 +361,29 @@ VH_DEV void join_row(const PagedAttnArgs &a, int64_t rh, int32_t gn, int32_t sn)
     store4(static_cast<T *>(a.out) + row * a.ld_out + (rh - row * a.heads) * a.c.hd + e, x * inv);
 }
 
+// The same for up to 64 segments, the tiles with the highest index first, whatever their segment: the last tiles of prompts see
+// the most keys, and what starts last should not take longest (24 prompts of 1 to 700 rows: 92 us segment by segment). Tiles
+// up to 2^23, whose sums are exact in f32.
+template <class F>
+VH_DEV bool find_tile_down(int32_t n, int32_t t, int32_t group, int32_t tile, F rows_of, int32_t *seg, int32_t *local) {
+    const int lane = threadIdx.x & 63;
+    const float mine = lane < n ? float(tiles_of(rows_of(lane), group, tile)) : 0.f;
+    auto from = [&](int32_t i) { return int32_t(wave_sum(fmaxf(mine - float(i), 0.f))); };  // tiles of index i and more
+    if (t >= from(0)) return false;
+    int32_t lo = 0, hi = int32_t(wave_max(mine));  // the index: the highest with from(index) > t
+    while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (from(mid) > t) lo = mid;
+        else hi = mid;
+    }
+    const uint64_t with = __ballot(mine > float(lo));
+    const int32_t rank = __popcll(with & ((uint64_t(1) << lane) - 1)), want = t - from(lo + 1);
+    const uint64_t at = __ballot((with >> lane & 1) && rank == want);
+    *seg = __ffsll(static_cast<unsigned long long>(at)) - 1;
+    *local = lo;
+    return at != 0;
+}
+
 // Softmax attention of a tile of query rows over a run of keys, on the matrix cores, transposed: S^T = K Q^T has a query row's
 // scores in the registers of one lane (two with 32 x 32 products, four with 16 x 16), so a row's maximum is a few register
 // maxima and one or two lane swaps, the rescale of O^T is by a lane's own factor, and P^T is already the operand that O^T +=
@@ -379,14 +433,12 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
         seg = group_segment(a.b, a.p, a.c.shift, seg_id);
         runs = runs_of(seg.key0, seg.key1, splits, a.gleast);
     } else {
-        t = a.stiles - 1 - t;  // the last tiles of a prompt see the most keys: first
-        seg_id = t;
-        if (!a.direct && !find_tile(a.b.seqs, t, group, TILE,
-                                    [&](int32_t i) {
-                                        const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
-                                        return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
-                                    },
-                                    &seg_id, &local))
+        auto rows_of = [&](int32_t i) {
+            const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
+            return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
+        };
+        if (!a.direct && !(a.b.seqs <= 64 && a.stiles <= 1 << 23 ? find_tile_down(a.b.seqs, t, group, TILE, rows_of, &seg_id, &local)
+                                                                 : find_tile(a.b.seqs, t, group, TILE, rows_of, &seg_id, &local)))
             return;
         const SeqRows sr = seq_rows(a.b, a.c.shift, seg_id);
         pf = a.prefix ? a.prefix[seg_id] : 0;
