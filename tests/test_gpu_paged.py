@@ -155,6 +155,44 @@ def test_append_without_q_and_many_sequences(hip):
             r.free()
 
 
+@pytest.mark.parametrize("wtype", TYPES, ids=IDS.get)
+@pytest.mark.parametrize("hd,heads,kv_heads,rot", [(64, 3, 1, 64), (128, 2, 2, 8), (24, 1, 1, 24)])
+def test_append_of_many_rows(hip, wtype, hd, heads, kv_heads, rot):
+    """As many rows as fill the chip, a wave each: 2048 and a few more, the last ones behind the last sequence."""
+    rows = [1000, 0, 1, 1047, 3]
+    b = Batch(rows, [1000, 5, 1, 1050, 3], wtype, heads, kv_heads, hd, 64, seed=7, pad_rows=2)
+    qd, kd = heads * hd, kv_heads * hd
+    x = b.normal(b.n_rows, qd + 2 * kd).to(ROW[wtype])
+    angle = torch.arange(1100, dtype=torch.float64)[:, None] * (1.0 / 1e4 ** (torch.arange(rot // 2) / (rot // 2)))[None]
+    rope = torch.stack([angle.cos(), angle.sin()], -1).float()
+    w = 1.0 + 0.1 * b.normal(hd)
+    r = Run(hip, b)
+    try:
+        dq = r.dev(torch.full((b.n_rows, qd), 5.0, dtype=ROW[wtype]))
+        hip.kv_append_dev(r.kv, r.batch, hip.append_rows(wtype, heads, r.dev(x), qd + 2 * kd, dq, qd, k_norm=r.dev(w), rope=r.dev(rope), rope_len=1100, rot_dim=rot))
+        hip.sync()
+        got_q, got_k, got_v = dq.get(), r.k.get(), r.v.get()
+        pos = torch.cat([torch.arange(l - n, l) for n, l in zip(rows, b.lens)])
+        n = pos.numel()
+        h = x[:n].view(n, heads + 2 * kv_heads, hd)
+        at = rope[pos]
+        tol = torch.full((), (hd + 16) * 2.0 ** -24 * 8, dtype=torch.float64)  # values below 8
+        assert off(got_q[:n].view(n, heads, hd), turned(h[:, :heads], None, 0, at, rot, False), tol, wtype) <= 1.0
+        assert bool((got_q[n:] == 5.0).all())
+        want_k = turned(h[:, heads:heads + kv_heads], w, 1e-6, at, rot, False)
+        row = 0
+        for s, (m, total) in enumerate(zip(rows, b.lens)):
+            for i in range(m):
+                for g in range(kv_heads):
+                    o = b.at(s, total - m + i, g)
+                    if i % 97 == 0 or i == m - 1:
+                        assert off(got_k[o:o + hd], want_k[row, g], tol, BF16 if wtype == BF16 else F16) <= 1.0, (s, i)
+                        assert torch.equal(got_v[o:o + hd], h[row, heads + kv_heads + g].to(CACHE[wtype])), (s, i)
+                row += 1
+    finally:
+        r.free()
+
+
 # ---------------------------------------------------------------- attention
 SHAPES = [(16, 8, 128), (14, 2, 64), (8, 8, 64), (5, 1, 80), (12, 4, 96), (32, 4, 128), (3, 3, 8), (40, 1, 32)]
 

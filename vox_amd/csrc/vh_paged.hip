@@ -7,6 +7,8 @@
 namespace vh {
 
 namespace {
+template <int N>
+using Int = std::integral_constant<int, N>;
 // Row type (WT_F32, WT_F16, WT_BF16) and cache type together: f32 and f16 rows read an f16 cache, bf16 rows a bf16 one.
 template <class F>
 hipError_t by_type(int type, F &&f) {
@@ -22,19 +24,24 @@ hipError_t launch_kv_append(int type, AppendArgs a, hipStream_t s) {
     // 8 values a lane (16 bytes of a 16-bit row) where a lane's pairs are one lane's too
     const bool wide = type != WT_F32 && (!a.rope || a.interleaved || a.rot % 16 == 0);
     const int lph = (a.c.hd <= 64 ? 16 : 32) / (wide ? 2 : 1), per = 256 / lph;
-    // turns of heads per row as blocks of their own up to about 2048 blocks (8 a CU), which hide each other's chains of reads
+    // Rows that fill the chip by themselves: a wave each. Fewer: a row's turns of heads as blocks of their own up to about 2048
+    // blocks (8 a CU).
+    const bool many = a.b.rows >= 2048;
     const int64_t turns = (a.heads + 2 * a.c.kv_heads + per - 1) / per;
     a.blocks = int32_t(std::max<int64_t>(1, std::min<int64_t>(turns, 2048 / a.b.rows)));
-    const int64_t grid = int64_t(a.b.rows) * a.blocks;
-    if (grid > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t grid = many ? (int64_t(a.b.rows) + 3) / 4 : int64_t(a.b.rows) * a.blocks;
     a.status = status_word();
     return by_type(type, [&](auto t, auto c) {
         using T = decltype(t);
         using C = decltype(c);
         const dim3 gr{unsigned(grid)}, bl{256};
+        auto go = [&](auto lanes, auto n) {
+            constexpr int L = decltype(lanes)::value, N = decltype(n)::value;
+            return many ? launch(k_kv_append<T, C, L, N, 64>, gr, bl, 0, s, a) : launch(k_kv_append<T, C, L, N, 256>, gr, bl, 0, s, a);
+        };
         if constexpr (!std::is_same<T, float>::value)
-            if (wide) return lph == 8 ? launch(k_kv_append<T, C, 8, 8>, gr, bl, 0, s, a) : launch(k_kv_append<T, C, 16, 8>, gr, bl, 0, s, a);
-        return lph == 16 ? launch(k_kv_append<T, C, 16, 4>, gr, bl, 0, s, a) : launch(k_kv_append<T, C, 32, 4>, gr, bl, 0, s, a);
+            if (wide) return lph == 8 ? go(Int<8>(), Int<8>()) : go(Int<16>(), Int<8>());
+        return lph == 16 ? go(Int<16>(), Int<4>()) : go(Int<32>(), Int<4>());
     });
 }
 

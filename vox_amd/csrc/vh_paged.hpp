@@ -48,14 +48,17 @@ VH_DEV void store4(T *p, f32x4 v) {
 }
 
 // One head of one row per LPH lanes, N neighbouring values a lane (16 bytes of a row where halves of the rotation allow it, else 4
-// values), 256 / LPH heads at a time; grid x = rows x a.blocks, block 256: block i of a row takes its heads in turns i, i +
-// a.blocks, ... (one each for a step's few rows, all of them where rows alone fill the chip: a block's chain of dependent
-// reads, not the bytes, is what a row costs). A lane of a rotated head also loads the N values its own are paired with
+// values), TPR / LPH heads at a time. What a row costs is its chain of dependent reads (its sequence, position, page and
+// rotation, then its values), so many rows are under way at once. TPR = 256: grid x = rows x a.blocks, block i of a row takes its
+// heads in turns i, i + a.blocks, ... (one each for a step's few rows). TPR = 64, for rows that fill the chip by themselves: a
+// wave a row, four rows a block, all heads in turns. A lane of a rotated head also loads the N values its own are paired with
 // (halves: rot / 2 away, in L1 by then; interleaved: among its own), so no value crosses lanes but the norm's sum. Rows behind
 // the last sequence, and rows at negative positions, write nothing.
-template <class T, class C, int LPH, int N>
+template <class T, class C, int LPH, int N, int TPR>
 __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
-    const int row = int(blockIdx.x) / a.blocks;
+    const int row = TPR == 64 ? int(blockIdx.x) * 4 + (int(threadIdx.x) >> 6) : int(blockIdx.x) / a.blocks;
+    if (TPR == 64 && row >= a.b.rows) return;
+    const int part = TPR == 64 ? 0 : int(blockIdx.x) % a.blocks, blocks = TPR == 64 ? 1 : a.blocks;
     const int e = N * (int(threadIdx.x) % LPH);
     const int hd = a.c.hd, G = a.c.kv_heads, heads = a.heads + 2 * G;
     const int32_t s = find_seq(a.b, row);
@@ -96,15 +99,15 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendArgs a) {
         }
     }
     const int pe = !inside || a.interleaved ? ec : low ? ec + half : ec - half;
-    constexpr int PER = 256 / LPH;
+    constexpr int PER = TPR / LPH;
     // the first values of the next turn are loaded during this one
-    auto head_of = [&](int turn) { return (int(blockIdx.x) % a.blocks + turn * a.blocks) * PER + int(threadIdx.x) / LPH; };
+    auto head_of = [&](int turn) { return (part + turn * blocks) * PER + int(threadIdx.x) % TPR / LPH; };
     auto values = [&](int turn, float (&x)[N], float (&xp)[N]) {
         const T *src = from + int64_t(min(head_of(turn), heads - 1)) * hd;
         load_n(src + ec, x);
         load_n(src + pe, xp);
     };
-    const int turns = ((heads + PER - 1) / PER + a.blocks - 1) / a.blocks;
+    const int turns = ((heads + PER - 1) / PER + blocks - 1) / blocks;
     float nx[N], np[N];
     values(0, nx, np);
     for (int k = 0; k < turns; ++k) {
