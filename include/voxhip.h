@@ -447,8 +447,8 @@ int voxhip_quantize_act_dev(const float *d_x, int64_t n, int8_t *d_xq, float *d_
  * serialise; the library's own workspace is shared by them all.
  *
  * Device contents are not checked by the host. A table entry that names no page of the pool, or row_start / len beyond the
- * buffers, touches nothing outside them: those keys are read as zeros, those rows not written or of no meaning, and the next
- * voxhip_sync (or synchronous call) fails. */
+ * buffers, touches nothing outside them: those keys are read as zeros, those rows not written or of no meaning (nor is
+ * what later calls write until then), and the next voxhip_sync (or synchronous call) fails. */
 /* One layer's pool: element d of kv head h at position p of a sequence lies at
  * page * page_stride + h * head_stride + (p % page_size) * pos_stride + d elements of k (and of v), page = the sequence's
  * table entry p / page_size. Both [pages][kv_heads][page_size][head_dim] and [pages][page_size][kv_heads][head_dim] (and wider
@@ -490,7 +490,8 @@ int voxhip_kv_append_dev(const voxhip_paged_kv *kv, const voxhip_paged_batch *b,
 /* Query rows q [rows][ld_q] and out [rows][ld_out] (may be q) of `heads` heads (a multiple of kv_heads), types as above.
  * The row at position p of a sequence sees the keys max(0, p - window + 1) (window 0: 0) .. min(len, max(p + 1, prefix[s])) - 1
  * and takes the mean of their values weighted by softmax of scale q.k, capped to cap tanh(. / cap) (cap 0: not), less
- * slopes[head] |p - key| (NULL: not). A row that sees no key gets zeros. */
+ * slopes[head] |p - key| (NULL: not). A row that sees no key gets zeros. Keys and values that a row does not see do not touch
+ * it, whatever they hold; a value that is not finite makes the rows that see it not finite in its place. */
 typedef struct voxhip_attn_rows {
     int32_t type, heads;
     const void *q;

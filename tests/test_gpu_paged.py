@@ -523,6 +523,31 @@ def test_bad_tables_are_reported(hip):
         r.free()
 
 
+def test_no_room_for_the_parts(hip):
+    """The attention's workspace refused by the memory limit: the call fails, the next one with room runs."""
+    n = 20000  # rows of 2 heads in 2 slots: 21 MB of parts, more than any other test here needs
+    b = Batch([1, 1], [40, 44], F16, 2, 1, 64, 16, [(0, 2, 32)], seed=3)
+    r = Run(hip, b)
+    big = r.dev(torch.zeros(n, 128, dtype=torch.float16))
+    batch = b.batch_struct(hip, r.bufs)
+    batch.rows = n
+    sh = hip.shared_prefix(1, 32, r.dev(torch.tensor([0, 2], dtype=torch.int32)), r.dev(torch.tensor([32], dtype=torch.int32)))
+    rows = hip.attn_rows(F16, 2, big, 128, big, 128, 0.125)
+    q = b.normal(2, 128).half()
+    before = r.attend(q)
+    try:
+        hip.lib().voxhip_set_vram_limit(hip.mem_info().used)
+        with pytest.raises(hip.VoxHipError, match="VRAM limit"):
+            hip.attn_shared_dev(r.kv, batch, sh, rows)
+        hip.lib().voxhip_set_vram_limit(0)
+        assert torch.equal(r.attend(q), before)  # the old workspace is gone; its like is made again
+        hip.attn_shared_dev(r.kv, batch, sh, rows)
+        hip.sync()
+    finally:
+        hip.lib().voxhip_set_vram_limit(0)
+        r.free()
+
+
 def test_range_of_f32_queries(hip):
     """A query beyond the f16 range, which the split of f32 rows cannot hold, is reported as elsewhere in the library."""
     b = Batch([1], [20], F32, 2, 1, 64, 16, seed=2)

@@ -148,6 +148,22 @@ def test_refusals(hip, oracle):
     hip.pool_free(pool)
 
 
+def test_no_room(hip, oracle):
+    """A pool that the memory limit refuses."""
+    mdl = Model(81, 1, 256, 4, 2, 64, 256, wtype=F16)
+    sv = Server(hip, mdl, 2)
+    try:
+        used = hip.mem_info().used
+        hip.lib().voxhip_set_vram_limit(used + (1 << 20))
+        with pytest.raises(hip.VoxHipError, match="VRAM limit"):
+            hip.pool_create(sv.xf, 4096, 128)
+        assert hip.mem_info().used == used
+    finally:
+        hip.lib().voxhip_set_vram_limit(0)
+    sv.step([3, 2])
+    hip.pool_free(sv.pool)
+
+
 def _one(hip):
     import ctypes as C
     keep = [np.array(v, np.int32) for v in ([1], [1], [0])]

@@ -270,20 +270,15 @@ VH_DEV float2 get_far(const float *p) {
     return float2{__uint_as_float(uint32_t(v)), __uint_as_float(uint32_t(v >> 32))};
 }
 
-// The group of sequence s (the first that holds it) and its shared keys, or -1 and 0: 64 groups at a time.
-VH_DEV int32_t find_group(const PagedGroups &p, int32_t s, int64_t most, int32_t *shared) {
+// The shared keys of the group that holds sequence s (the first that does; none: 0): 64 groups at a time.
+VH_DEV int32_t shared_keys(const PagedGroups &p, int32_t s, int64_t most) {
     const int lane = threadIdx.x & 63;
     for (int32_t base = 0; base < p.groups; base += 64) {
         const int32_t g = min(base + lane, p.groups - 1), n = p.len[g];
         const uint64_t in = __ballot(base + lane < p.groups && s >= p.seq_start[g] && s < p.seq_start[g + 1]);
-        if (in) {
-            const int l = __ffsll(static_cast<unsigned long long>(in)) - 1;
-            *shared = clamp_i32(__builtin_amdgcn_readlane(n, l), 0, most);
-            return base + l;
-        }
+        if (in) return clamp_i32(__builtin_amdgcn_readlane(n, __ffsll(static_cast<unsigned long long>(in)) - 1), 0, most);
     }
-    *shared = 0;
-    return -1;
+    return 0;
 }
 
 // The segment (of n, with rows_of(i) rows each) and the tile in it of the launch's tile t: 64 segments at a time.
@@ -426,13 +421,18 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
     const int g = id % G;
     id /= G;
     const int split = id % splits;
-    int32_t t = id / splits, seg_id = t, local = 0, shared = 0;
+    int32_t t = id / splits, seg_id = t, local = 0, shared = 0;  // shared: of a sequence, the keys of its group
     Segment seg;
     bool whole = false;  // rows whose keys are one run are written here, otherwise the last block of a row joins its parts
     int32_t gruns = 0, pf = 0;
     Runs runs;
     if constexpr (GROUPS) {
-        if (!find_tile(a.p.groups, t, group, TILE, [&](int32_t i) { return group_segment(a.b, a.p, a.c.shift, i).rows; }, &seg_id, &local)) return;
+        if (a.p.groups == 1) {  // nothing to look for: a round trip less
+            seg_id = 0;
+            local = t;
+        } else if (!find_tile(a.p.groups, t, group, TILE, [&](int32_t i) { return group_segment(a.b, a.p, a.c.shift, i).rows; }, &seg_id, &local)) {
+            return;
+        }
         seg = group_segment(a.b, a.p, a.c.shift, seg_id);
         runs = runs_of(seg.key0, seg.key1, splits, a.gleast);
     } else {
@@ -440,13 +440,15 @@ VH_DEV void attn_tile(const PagedAttnArgs &a, int id, uint8_t *smem) {
             const int32_t r0 = clamp_i32(a.b.row_start[i], 0, a.b.rows);
             return clamp_i32(a.b.row_start[i + 1], r0, a.b.rows) - r0;
         };
-        if (!a.direct && !(a.b.seqs <= 64 && a.stiles <= 1 << 23 ? find_tile_down(a.b.seqs, t, group, TILE, rows_of, &seg_id, &local)
+        if (!a.direct && a.b.seqs == 1) {
+            seg_id = 0;
+            local = a.stiles - 1 - t;
+        } else if (!a.direct && !(a.b.seqs <= 64 && a.stiles <= 1 << 23 ? find_tile_down(a.b.seqs, t, group, TILE, rows_of, &seg_id, &local)
                                                                  : find_tile(a.b.seqs, t, group, TILE, rows_of, &seg_id, &local)))
             return;
-        const SeqRows sr = seq_rows(a.b, a.c.shift, seg_id);
         pf = a.prefix ? a.prefix[seg_id] : 0;
-        find_group(a.p, seg_id, a.b.page_ld << a.c.shift, &shared);
-        seg = Segment{sr.first, sr.n, seg_id, seg_id + 1, min(shared, sr.len), sr.len, sr.ok};
+        shared = shared_keys(a.p, seg_id, a.b.page_ld << a.c.shift);
+        seg = seq_segment(a.b, a.c.shift, seg_id, shared);
         runs = runs_of(seg.key0, seg.key1, splits, a.sleast);
     }
     const int32_t qrows = seg.rows * group;

@@ -69,13 +69,6 @@ VH_HD int64_t key_offset(const PagedKv &c, int32_t page, int32_t head, int32_t p
     return int64_t(page) * c.page_stride + int64_t(head) * c.head_stride + int64_t(pos & ((1 << c.shift) - 1)) * c.pos_stride;
 }
 
-// The group of sequence s, or -1. A group's bounds are clamped to the batch's sequences.
-VH_HD int32_t group_of(const PagedGroups &p, int32_t s) {
-    for (int32_t g = 0; g < p.groups; ++g)
-        if (s >= p.seq_start[g] && s < p.seq_start[g + 1]) return g;
-    return -1;
-}
-
 // ------------------------------------------------------------------ the attention's work
 // A segment is what meets one run of keys: the rows of a group and its shared keys, or the rows of a sequence and its own
 // keys behind the shared ones. Its query rows are (row, head of the kv head's `group` heads), the head fastest; a tile is
@@ -97,9 +90,9 @@ VH_HD Segment group_segment(const PagedBatch &b, const PagedGroups &p, int32_t s
     s.ok = s.seq0 == p.seq_start[g] && s.seq1 == p.seq_start[g + 1] && s.key1 == p.len[g];
     return s;
 }
-VH_HD Segment seq_segment(const PagedBatch &b, const PagedGroups &p, int32_t shift, int32_t seq) {
+// shared: the keys of the sequence's group (0: none).
+VH_HD Segment seq_segment(const PagedBatch &b, int32_t shift, int32_t seq, int32_t shared) {
     const SeqRows r = seq_rows(b, shift, seq);
-    const int32_t g = group_of(p, seq), shared = g >= 0 ? p.len[g] : 0;
     Segment s;
     s.seq0 = seq;
     s.seq1 = seq + 1;
