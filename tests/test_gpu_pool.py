@@ -94,6 +94,15 @@ def test_quantized_prompts(hip, oracle):
     hip.pool_free(sv.pool)
 
 
+def test_more_sessions_than_the_head_takes_at_once(hip, oracle):
+    # a q4 head takes 8 rows a product; f16 layers take all 21 sessions' rows in one pass
+    mdl = Model(57, 1, 256, 4, 2, 64, 256, wtype=F16, head_rows=96, head_type=Q4)
+    sv = Server(hip, mdl, 21, pages=128, cap=60)
+    sv.step([2] * 20 + [30])
+    sv.step([1] * 21)
+    hip.pool_free(sv.pool)
+
+
 @pytest.mark.parametrize("wt", [F32, F16])
 def test_shared_prompt(hip, oracle, wt):
     """One session of each voice reads the prompt, the others begin behind its whole pages (32 of 37 keys of the second voice's);

@@ -4207,7 +4207,7 @@ int forward_paged(int xfmr, int pool, const voxhip_pool_batch *b, const float *x
     for (const LayerDev &L : X.L)
         for (int id : {L.qkv, L.o, L.gu, L.down}) chunk = std::min(chunk, rows_per_pass(g.mats[size_t(id)], total));
     const int64_t V = head >= 0 ? mat_at(head).rows : 0;
-    if (head >= 0) chunk = std::min(chunk, rows_per_pass(mat_at(head), n_out));
+    const int head_rows = head >= 0 ? rows_per_pass(mat_at(head), n_out) : kMaxPass;  // of one product with the head
     chunk = int(std::min<int64_t>(chunk, total));
     ensure_rows(X, chunk);
     const OnDevice on;
@@ -4277,16 +4277,19 @@ int forward_paged(int xfmr, int pool, const voxhip_pool_batch *b, const float *x
         enqueue_layers_paged(X, P, pb, pg, max_rows, max_len, max_shared, total, g.stream);
         const int mr = int(ends.size());
         if (mr && (out || head >= 0)) {
-            if (head >= 0) prepare_mat(mat_at(head), n_out, mr, g.stream);
             HIPCHECK(launch_gather_rows(X.h, H, g.paged_meta + (pick - g.paged_meta_host), mr, X.pre, g.stream));
-            enqueue_final(X, 0, mr, head, g.stream, X.pre, n_out);
-            auto give = [&](const float *dev, int64_t w, float *to) {
-                HIPCHECK(copy_d2h(pin, dev, size_t(mr) * size_t(w) * 4, g.stream));
-                HIPCHECK(hipStreamSynchronize(g.stream));
-                for (int i = 0; i < mr; ++i) std::memcpy(to + int64_t(ends[size_t(i)]) * w, pin + int64_t(i) * w, size_t(w) * 4);
-            };
-            if (out) give(X.xnorm, H, out);
-            if (head >= 0 && head_out) give(X.logits, V, head_out);
+            for (int e0 = 0; e0 < mr; e0 += head_rows) {
+                const int n = std::min(head_rows, mr - e0);
+                if (head >= 0) prepare_mat(mat_at(head), n_out, n, g.stream);
+                enqueue_final(X, 0, n, head, g.stream, X.pre + int64_t(e0) * H, n_out);
+                auto give = [&](const float *dev, int64_t w, float *to) {
+                    HIPCHECK(copy_d2h(pin, dev, size_t(n) * size_t(w) * 4, g.stream));
+                    HIPCHECK(hipStreamSynchronize(g.stream));
+                    for (int i = 0; i < n; ++i) std::memcpy(to + int64_t(ends[size_t(e0 + i)]) * w, pin + int64_t(i) * w, size_t(w) * 4);
+                };
+                if (out) give(X.xnorm, H, out);
+                if (head >= 0 && head_out) give(X.logits, V, head_out);
+            }
         }
         at += mc;
     }
