@@ -536,7 +536,7 @@ def test_no_room_for_the_parts(hip):
     q = b.normal(2, 128).half()
     before = r.attend(q)
     try:
-        hip.lib().voxhip_set_vram_limit(hip.mem_info().used)
+        hip.lib().voxhip_set_vram_limit(1)  # less than any weight copies of other tests' models, which would give way, can make room for
         with pytest.raises(hip.VoxHipError, match="VRAM limit"):
             hip.attn_shared_dev(r.kv, batch, sh, rows)
         hip.lib().voxhip_set_vram_limit(0)
